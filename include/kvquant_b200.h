@@ -342,6 +342,110 @@ int kvq_fit_codebook(const float* x, const float* weights, int64_t n, int bits,
 int kvq_set_decode_kernels(int key_kernel, int value_kernel);
 int kvq_decode_kernels(void);
 
+/* ---------------------------------------------------------------------------
+ * Paged 8-bit KV cache (no counterpart in the reference, whose cache is one
+ * contiguous slot per layer, kvquant/kv_cache.py:4-44).
+ *
+ *   pool     uint8 [n_pages, n_heads, page_tokens / 16, 32 * D + 16] per layer,
+ *            16-byte aligned. A record is 16 tokens (t) of one KV head, D = 64 or
+ *            128 channels (d): key codes in the order [d/32][t%8][(d/4)%4]
+ *            [(d/16)%2][t/8][d%4], value codes [d/32][d%8][(t/2)%4][(d/16)%2]
+ *            [(d/8)%2][t/8][t%2], the fp32 key scale and value scale, 8 zero
+ *            bytes. kind 0 (int8): byte = code + 128, code in -127..127; kind 1:
+ *            the e4m3 float. Value = code * scale. page_tokens: a multiple of 16,
+ *            at most 1024.
+ *   table    int32 [n_slots, n_cols]: a slot's pages in token order, -1 = none.
+ *   lengths  int32 [n_slots]: a slot's tokens.
+ *   refs     int32 [n_pages]: how many slots hold a page.
+ *   slots    int32 [B]: the slot of each of the call's B (1..4096) sequences, all
+ *            different; NULL: 0, 1, .. B - 1.
+ *   indptr   int32 [B + 1]: the call's rows of each sequence, of `total`; NULL:
+ *            total / B each. Rows of append and attention are a slot's last
+ *            tokens (lengths already counts them).
+ * Pages, slots, lengths and row ranges that are out of range are skipped and
+ * make kvq_check_status() fail; nothing outside the given arrays is touched.
+ * dtype: 0 = fp16, 1 = bf16, 2 = fp32 (outputs of kvq_paged_read only).
+ * Strides are in elements.
+ * ------------------------------------------------------------------------- */
+
+/* Writes the new tokens' k and v rows [total, n_heads, D] (16-byte aligned rows).
+ * A block started by the call gets scale = max(max|x| / Q, 2^-32) over its new
+ * tokens (Q = 127 or 448; finite x only), code = round-to-even(x * (1 / scale));
+ * infinities become the largest code, NaN 0. An open block keeps the larger of
+ * its scale and that one and, when it grew, its codes become
+ * round(code * (old scale * (1 / scale))). Places after the last token hold 0. */
+int kvq_paged_append(const void* k, int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+                     int64_t v_tok_stride, int64_t v_head_stride, int dtype, uint8_t* pool,
+                     int kind, int64_t n_pages, int64_t n_heads, int64_t head_dim,
+                     int64_t page_tokens, const int32_t* table, int64_t n_slots, int64_t n_cols,
+                     const int32_t* lengths, const int32_t* slots, const int32_t* indptr,
+                     int64_t B, int64_t total, void* stream);
+
+/* Values of the tokens [starts[b], starts[b] + rows of b) (starts NULL: 0) as
+ * k_out, v_out [total, n_heads, D] of `dtype`. */
+int kvq_paged_read(const uint8_t* pool, int kind, int64_t n_pages, int64_t n_heads,
+                   int64_t head_dim, int64_t page_tokens, const int32_t* table, int64_t n_slots,
+                   int64_t n_cols, const int32_t* lengths, const int32_t* slots,
+                   const int32_t* starts, const int32_t* indptr, int64_t B, int64_t total,
+                   void* k_out, void* v_out, int dtype, void* stream);
+
+/* Causal attention of the new tokens' queries q [total, n_heads * group, D]
+ * (16-byte aligned rows) over their slots' tokens: out [total, n_heads * group,
+ * D] in q's type; a row at position p sees the tokens j <= p, with window > 0
+ * only j > p - window; a row that sees none is 0. ml_out: NULL or fp32 pairs
+ * [total, n_heads * group] = (M, 1 / L) of softmax(scores * scale), (-inf, inf)
+ * for such a row (kvq_merge_shards takes them). group <= 64; max_new: the most
+ * rows of any sequence (a sequence with more is skipped and flagged). */
+size_t kvq_paged_attention_workspace(int64_t head_dim, int64_t max_new, int64_t group);
+int kvq_paged_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int dtype,
+                        int64_t group, const uint8_t* pool, int kind, int64_t n_pages,
+                        int64_t n_heads, int64_t head_dim, int64_t page_tokens,
+                        const int32_t* table, int64_t n_slots, int64_t n_cols,
+                        const int32_t* lengths, const int32_t* slots, const int32_t* indptr,
+                        int64_t B, int64_t total, int64_t max_new, float scale, int64_t window,
+                        void* out, float* ml_out, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* Page operations, n <= 4096 slots a call. status: int32 (device), bits are only
+ * ever set: 1 = no free pages left, 2 = a slot that the operation cannot take.
+ * free: the slots' rows become -1, their lengths 0, their pages' refs go down
+ * (a slot out of range or named before in the list is skipped, bit 2). */
+int kvq_paged_free(int32_t* table, int64_t n_slots, int64_t n_cols, int32_t* lengths,
+                   int32_t* refs, int64_t n_pages, int64_t page_tokens, const int32_t* slots,
+                   int64_t n, int32_t* status, void* stream);
+/* fork: dst[i] shares all pages of src[i]. A pair whose dst holds tokens, is one
+ * of src, is named before or is out of range is skipped (bit 2). */
+int kvq_paged_fork(int32_t* table, int64_t n_slots, int64_t n_cols, int32_t* lengths,
+                   int32_t* refs, int64_t n_pages, int64_t page_tokens, const int32_t* src,
+                   const int32_t* dst, int64_t n, int32_t* status, void* stream);
+/* extend: room for n_new[i] (NULL: n_new_all) more tokens in slots[i], lengths
+ * grow; free pages (refs 0) are taken in ascending order, slot after slot. A
+ * slot whose last page is open and shared gets a copy of it in every layer
+ * (pool: n_layers of n_pages pages, layer_stride bytes apart) unless all its
+ * other holders stand before it in the list. All or nothing: without enough
+ * pages (bit 1), or with a slot out of range, named twice or too long for its
+ * row (bit 2), nothing changes. */
+size_t kvq_paged_extend_workspace(int64_t n_pages);
+int kvq_paged_extend(uint8_t* pool, int64_t n_layers, int64_t layer_stride, int64_t page_bytes,
+                     int32_t* table, int64_t n_slots, int64_t n_cols, int32_t* lengths,
+                     int32_t* refs, int64_t n_pages, int64_t page_tokens, const int32_t* slots,
+                     int64_t n, const int32_t* n_new, int64_t n_new_all, int32_t* status,
+                     void* workspace, size_t workspace_bytes, void* stream);
+/* compact: with L live pages (refs > 0), those with ids >= L move in ascending
+ * order into the free ids below L, in every layer; table and refs follow, L goes
+ * to *n_live (device). Workspace: kvq_paged_extend_workspace(n_pages). */
+int kvq_paged_compact(uint8_t* pool, int64_t n_layers, int64_t layer_stride, int64_t page_bytes,
+                      int32_t* table, int64_t n_slots, int64_t n_cols, int32_t* refs,
+                      int64_t n_pages, int32_t* n_live, void* workspace, size_t workspace_bytes,
+                      void* stream);
+/* copy: pages src[i] of one pool to pages dst[i] of another or the same one,
+ * every layer. The dst pages are distinct and, in one pool, none is in src. */
+size_t kvq_paged_copy_workspace(int64_t n);
+int kvq_paged_copy(const uint8_t* src_pool, int64_t src_pages, int64_t src_layer_stride,
+                   uint8_t* dst_pool, int64_t dst_pages, int64_t dst_layer_stride,
+                   int64_t n_layers, int64_t page_bytes, const int32_t* src, const int32_t* dst,
+                   int64_t n, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Reads and clears the device-side error flag set by kernels that skip
  * out-of-range accesses (synchronizes `stream`). */
 int kvq_check_status(void* stream);

@@ -8,3 +8,5 @@
 #include "kvq_decode.cuh"
 #include "kvq_noalloc.cuh"
 #include "kvq_codebook.cuh"
+#include "kvq_paged.cuh"
+#include "kvq_paged_attn.cuh"

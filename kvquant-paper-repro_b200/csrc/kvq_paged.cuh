@@ -1,0 +1,1140 @@
+// Paged 8-bit KV cache: the record format, append, read, and the page operations
+// (fork, extend with copy-on-write, free, compact, copy). The attention that
+// reads the cache is in kvq_paged_attn.cuh. Part of the kvq_lib.cu unity build.
+//
+// A block is 16 tokens of one KV head and is one record of 32 * D + 16 bytes:
+//   key codes [D/32][t%8][(d/4)%4][(d/16)%2][t/8][d%4]
+//   value codes [D/32][d%8][(t/2)%4][(d/16)%2][(d/8)%2][t/8][t%2]
+//   key scale, value scale (fp32), 8 zero bytes
+// The byte order is that of the A fragments of mma.m16n8k16: lane 4g + c of a
+// warp reads its share of both operands as D/32 16-byte words at 16 * lane,
+// coalesced and free of bank conflicts, and no code moves between lanes. A
+// record is one contiguous copy, scales included; a page (its blocks of every
+// head) is one contiguous copy too.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+#include <type_traits>
+
+#include "kvq_common.cuh"
+#include "kvq_sm100.cuh"
+
+namespace kvq {
+namespace paged {
+
+constexpr int kBlock = 16;                    // tokens per record
+constexpr float kScaleFloor = 0x1p-32f;       // least scale of a block
+constexpr int kMaxSeqs = 4096;                // sequences (or slots) per call
+enum Kind : int { kInt8 = 0, kE4m3 = 1 };
+enum StatusBit : int { kNoPages = 1, kBadSlot = 2 };  // bits of the page operations' status
+
+__host__ __device__ constexpr int rec_bytes(int D) { return 32 * D + 16; }
+
+// The cache as one call sees it: a layer's pool, the page table and the call's
+// sequences (rows of the table, with their shares of the call's token rows).
+struct View {
+  uint8_t* pool;
+  int64_t n_pages;
+  int heads, dim, blocks;      // blocks per page
+  const int32_t* table;        // [n_slots, n_cols]
+  int64_t n_slots, n_cols;
+  const int32_t* lengths;      // [n_slots]
+  const int32_t* slots;        // [B] or null: sequence b is slot b
+  const int32_t* indptr;       // [B + 1] or null: total / B rows each
+  int64_t B, total;
+
+  __host__ __device__ int64_t head_bytes() const { return (int64_t)blocks * rec_bytes(dim); }
+  __host__ __device__ int64_t page_bytes() const { return heads * head_bytes(); }
+
+  // Sequence b's slot (-1: out of range, flagged).
+  __device__ int slot(int64_t b) const {
+    const int s = slots ? slots[b] : (int)b;
+    if (s < 0 || s >= n_slots) {
+      atomicOr(&g_status, kStatusBadIndex);
+      return -1;
+    }
+    return s;
+  }
+  // Tokens of a slot (0 and flagged when its row cannot hold them).
+  __device__ int length(int s) const {
+    const int n = lengths[s];
+    if (n < 0 || n > n_cols * blocks * kBlock) {
+      atomicOr(&g_status, kStatusBadIndex);
+      return 0;
+    }
+    return n;
+  }
+  // Rows [r0, r1) of the call that belong to sequence b (none and flagged when out of range).
+  __device__ void rows(int64_t b, int64_t& r0, int64_t& r1) const {
+    if (!indptr) {
+      const int64_t n = total / B;
+      r0 = b * n;
+      r1 = r0 + n;
+      return;
+    }
+    r0 = indptr[b];
+    r1 = indptr[b + 1];
+    if (r0 < 0 || r1 < r0 || r1 > total) {
+      atomicOr(&g_status, kStatusBadIndex);
+      r0 = r1 = 0;
+    }
+  }
+  // Record of block `blk` of slot s, head h (null and flagged without a page).
+  __device__ uint8_t* record(int s, int blk, int h) const {
+    const int page = table[(int64_t)s * n_cols + blk / blocks];
+    if (page < 0 || page >= n_pages) {
+      atomicOr(&g_status, kStatusBadIndex);
+      return nullptr;
+    }
+    return pool + page * page_bytes() + h * head_bytes() +
+           (int64_t)(blk % blocks) * rec_bytes(dim);
+  }
+};
+
+// Items of a call over the 16-token blocks that its rows touch: sequence b gets
+// the items [indptr[b] / 16 + 2 b, indptr[b + 1] / 16 + 2 (b + 1)). m rows touch
+// at most (m + 14) / 16 + 1 blocks wherever they start, which is never more than
+// that range holds, so no prefix sum over the sequences is needed: an item finds
+// its sequence by a search whose steps probe 32 places at once.
+inline int64_t block_items(const View& v) {
+  return v.indptr ? v.total / kBlock + 2 * v.B : v.B * (v.total / v.B / kBlock + 2);
+}
+__device__ __forceinline__ void find_item(const View& v, int64_t item, int lane, int64_t& b,
+                                          int64_t& local) {
+  if (!v.indptr) {
+    const int64_t per = v.total / v.B / kBlock + 2;
+    b = item / per;
+    local = item % per;
+    return;
+  }
+  int64_t lo = 0, hi = v.B;
+  while (hi - lo > 1) {
+    const int64_t step = (hi - lo + 31) / 32;
+    const int64_t i = lo + (lane + 1) * step;
+    const bool below = i < hi && v.indptr[i] / kBlock + 2 * i <= item;
+    lo += step * __popc(__ballot_sync(0xffffffffu, below));
+    hi = min(hi, lo + step);
+  }
+  b = lo;
+  local = item - (v.indptr[lo] / kBlock + 2 * lo);
+}
+
+template <typename T>
+__device__ __forceinline__ float2 to_float2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 to_float2<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <>
+__device__ __forceinline__ float2 to_float2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t from_float2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t from_float2<__half>(float a, float b) {
+  return half2_bits(a, b);
+}
+template <>
+__device__ __forceinline__ uint32_t from_float2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int KIND>
+struct Code;
+template <>
+struct Code<kInt8> {
+  static constexpr float kMax = 127.f;
+  static constexpr uint32_t kZero = 0x80808080u;  // four codes of 0
+  // Four codes from values already divided by the scale; NaN gives 0.
+  static __device__ __forceinline__ uint32_t pack(float a, float b, float c, float d) {
+    auto q = [](float x) { return (uint32_t)(max(-127, min(127, __float2int_rn(x))) + 128); };
+    return prmt(prmt(q(a), q(b), 0x0040), prmt(q(c), q(d), 0x0040), 0x5410);
+  }
+  static __device__ __forceinline__ void unpack(uint32_t w, float (&x)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = (float)(int)((w >> (8 * e)) & 0xffu) - 128.f;
+  }
+};
+template <>
+struct Code<kE4m3> {
+  static constexpr float kMax = 448.f;
+  static constexpr uint32_t kZero = 0u;
+  static __device__ __forceinline__ uint32_t pack(float a, float b, float c, float d) {
+    auto two = [](float x, float y) {
+      x = x == x ? x : 0.f;
+      y = y == y ? y : 0.f;
+      uint16_t r;
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(y), "f"(x));
+      return (uint32_t)r;
+    };
+    return two(a, b) | (two(c, d) << 16);
+  }
+  static __device__ __forceinline__ void unpack(uint32_t w, float (&x)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      uint32_t h;
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(w >> (8 * e))));
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      x[e] = f.x;
+      x[e + 1] = f.y;
+    }
+  }
+};
+
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a < INFINITY ? a : 0.f;  // NaN and the infinities do not set a scale
+}
+
+// Which channels and tokens a lane handles when rows of tokens are turned into a
+// record or back, and where its words lie. Both maps read and write token rows
+// in 16-byte words (8 channels).
+//   keys: word `w` (channels 8x + 4w ..) of token t; the lane bits are chosen so
+//   that the 32 words of one access fall into 32 banks.
+//   values: the four tokens of one code word, 8 channels e.
+struct KeyMap {
+  int jj, xh, g01, r, swap;
+  __device__ explicit KeyMap(int lane)
+      : jj(lane & 1), xh((lane >> 1) & 1), g01(((lane >> 2) & 1) | ((lane >> 4) & 1) << 1),
+        r((lane >> 3) & 1), swap((lane >> 4) & 1) {}
+  // step: i * 2 + (g >> 2)
+  __device__ int token(int step) const { return g01 + 4 * (step & 1) + 8 * r; }
+  __device__ int channel(int step) const { return 32 * (step >> 1) + 16 * jj + 8 * xh; }
+  __device__ int offset(int step, int w) const {
+    return 512 * (step >> 1) + 64 * (g01 + 4 * (step & 1)) + 16 * (2 * xh + w) + 8 * jj + 4 * r;
+  }
+};
+struct ValueMap {
+  int c, y0;
+  __device__ explicit ValueMap(int lane) : c(lane & 3), y0(lane >> 2) {}
+  __device__ int token(int e) const { return 2 * c + (e & 1) + 8 * (e >> 1); }
+  __device__ int channel(int step) const { return 8 * (y0 + 8 * step); }
+  __device__ int offset(int step, int e) const {
+    const int y = y0 + 8 * step;
+    return 512 * (y >> 2) + 64 * e + 16 * c + 8 * ((y >> 1) & 1) + 4 * (y & 1);
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Append
+// ---------------------------------------------------------------------------
+// One warp per (touched block, head). A block started by the call gets
+//   s = max(max|x| / Qmax, 2^-32), code = round(x / s) (as x times 1 / s),
+// an open block keeps the larger of its scale and that, and its older codes are
+// restated as round(code * s_old / s) when it grew: at most half a step of the
+// new scale of error each time. Places past the last token hold the code 0.
+// Bound by HBM: 4 D bytes in and 2 D + 1 bytes out per token and head.
+constexpr int kAppendWarps = 4;
+
+template <int D, int KIND, typename T>
+__global__ void __launch_bounds__(32 * kAppendWarps) append_kernel(
+    View v, const T* __restrict__ k, int64_t k_tok, int64_t k_head, const T* __restrict__ val,
+    int64_t v_tok, int64_t v_head, int64_t n_warps) {
+  constexpr int R = rec_bytes(D), NC = D / 16;  // NC: 16-byte words of a lane, K or V
+  using C = Code<KIND>;
+  __shared__ __align__(128) uint8_t smem[kAppendWarps][(R + 127) / 128 * 128];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int64_t warp = (int64_t)blockIdx.x * kAppendWarps + wid;
+  if (warp >= n_warps) return;
+  const int h = (int)(warp % v.heads);
+  int64_t b, local;
+  find_item(v, warp / v.heads, lane, b, local);
+  const int s = v.slot(b);
+  if (s < 0) return;
+  int64_t r0, r1;
+  v.rows(b, r0, r1);
+  const int len = v.length(s);
+  const int start = len - (int)(r1 - r0);
+  if (r1 == r0) return;
+  if (start < 0) {  // more new tokens than the slot holds
+    atomicOr(&g_status, kStatusBadIndex);
+    return;
+  }
+  const int64_t blk64 = start / kBlock + local;
+  if (local < 0 || blk64 * kBlock >= len) return;
+  const int t0 = (int)blk64 * kBlock;
+  uint8_t* rec = v.record(s, (int)blk64, h);
+  if (!rec) return;
+  uint8_t* sm = smem[wid];
+
+  // token t of the block is new when first <= t < last
+  const int first = max(0, start - t0), last = min(kBlock, len - t0);
+  const T* kp = k + (r0 + t0 - start) * k_tok + h * k_head;
+  const T* vp = val + (r0 + t0 - start) * v_tok + h * v_head;
+  const KeyMap km(lane);
+  const ValueMap vm(lane);
+  uint4 kx[NC], vx[NC];
+  float ka = 0.f, va = 0.f;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int t = km.token(i);
+    kx[i] = make_uint4(0, 0, 0, 0);
+    if (t >= first && t < last)
+      kx[i] = *reinterpret_cast<const uint4*>(kp + t * k_tok + km.channel(i));
+    const int tv = vm.token(i & 3);
+    vx[i] = make_uint4(0, 0, 0, 0);
+    if (tv >= first && tv < last)
+      vx[i] = *reinterpret_cast<const uint4*>(vp + tv * v_tok + vm.channel(i >> 2));
+  }
+  float ks_old = 0.f, vs_old = 0.f;
+  if (first > 0) {
+    for (int o = lane * 16; o < R; o += 512)
+      *reinterpret_cast<uint4*>(sm + o) = *reinterpret_cast<const uint4*>(rec + o);
+    __syncwarp();
+    ks_old = *reinterpret_cast<const float*>(sm + 32 * D);
+    vs_old = *reinterpret_cast<const float*>(sm + 32 * D + 4);
+  }
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const uint32_t kw[4] = {kx[i].x, kx[i].y, kx[i].z, kx[i].w};
+    const uint32_t vw[4] = {vx[i].x, vx[i].y, vx[i].z, vx[i].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 a = to_float2<T>(kw[e]), c = to_float2<T>(vw[e]);
+      ka = fmaxf(ka, fmaxf(finite_abs(a.x), finite_abs(a.y)));
+      va = fmaxf(va, fmaxf(finite_abs(c.x), finite_abs(c.y)));
+    }
+  }
+  const float ks = fmaxf(ks_old, fmaxf(__fmul_rn(warp_max(ka), 1.f / C::kMax), kScaleFloor));
+  const float vs = fmaxf(vs_old, fmaxf(__fmul_rn(warp_max(va), 1.f / C::kMax), kScaleFloor));
+  const float ki = __fdiv_rn(1.f, ks), vi = __fdiv_rn(1.f, vs);
+
+  if (first > 0) {
+    // older codes: restated when the scale grew; the places after them: 0
+    const float kf = __fmul_rn(ks_old, ki), vf = __fmul_rn(vs_old, vi);
+    for (int o = lane * 4; o < 32 * D; o += 128) {
+      uint32_t w = *reinterpret_cast<const uint32_t*>(sm + o);
+      const bool key = o < 16 * D;
+      if (key ? ks > ks_old : vs > vs_old) {
+        float x[4];
+        C::unpack(w, x);
+        const float f = key ? kf : vf;
+        w = C::pack(__fmul_rn(x[0], f), __fmul_rn(x[1], f), __fmul_rn(x[2], f),
+                    __fmul_rn(x[3], f));
+      }
+      uint32_t keep = 0;
+      if (key) {
+        keep = ((o >> 6) & 7) + 8 * ((o >> 2) & 1) < first ? 0xffffffffu : 0u;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (2 * ((o >> 4) & 3) + (e & 1) + 8 * (e >> 1) < first) keep |= 0xffu << (8 * e);
+      }
+      *reinterpret_cast<uint32_t*>(sm + o) = (w & keep) | (C::kZero & ~keep);
+    }
+    __syncwarp();
+  }
+
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int t = km.token(i);
+    const uint32_t xw[4] = {kx[i].x, kx[i].y, kx[i].z, kx[i].w};
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const int ww = w ^ km.swap;
+      const uint32_t x0 = ww ? xw[2] : xw[0], x1 = ww ? xw[3] : xw[1];
+      const float2 a = to_float2<T>(x0), c = to_float2<T>(x1);
+      const uint32_t code = C::pack(__fmul_rn(a.x, ki), __fmul_rn(a.y, ki), __fmul_rn(c.x, ki),
+                                    __fmul_rn(c.y, ki));
+      if (first == 0 || (t >= first && t < last))
+        *reinterpret_cast<uint32_t*>(sm + km.offset(i, ww)) = code;
+    }
+  }
+  uint32_t fresh = 0;  // bytes of a value word that are new tokens
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (vm.token(e) >= first && vm.token(e) < last) fresh |= 0xffu << (8 * e);
+#pragma unroll
+  for (int i = 0; i < NC; i += 4) {
+    const uint32_t* x0 = reinterpret_cast<const uint32_t*>(&vx[i]);
+    const uint32_t* x1 = reinterpret_cast<const uint32_t*>(&vx[i + 1]);
+    const uint32_t* x2 = reinterpret_cast<const uint32_t*>(&vx[i + 2]);
+    const uint32_t* x3 = reinterpret_cast<const uint32_t*>(&vx[i + 3]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float2 a = to_float2<T>(x0[e >> 1]), bb = to_float2<T>(x1[e >> 1]);
+      const float2 c = to_float2<T>(x2[e >> 1]), d = to_float2<T>(x3[e >> 1]);
+      const uint32_t code =
+          (e & 1) ? C::pack(__fmul_rn(a.y, vi), __fmul_rn(bb.y, vi), __fmul_rn(c.y, vi),
+                            __fmul_rn(d.y, vi))
+                  : C::pack(__fmul_rn(a.x, vi), __fmul_rn(bb.x, vi), __fmul_rn(c.x, vi),
+                            __fmul_rn(d.x, vi));
+      uint32_t* at = reinterpret_cast<uint32_t*>(sm + 16 * D + vm.offset(i >> 2, e));
+      *at = first == 0 ? code : (*at & ~fresh) | (code & fresh);
+    }
+  }
+  if (lane < 4)
+    *reinterpret_cast<float*>(sm + 32 * D + 4 * lane) = lane == 0 ? ks : lane == 1 ? vs : 0.f;
+  __syncwarp();
+  for (int o = lane * 16; o < R; o += 512)
+    *reinterpret_cast<uint4*>(rec + o) = *reinterpret_cast<const uint4*>(sm + o);
+}
+
+// ---------------------------------------------------------------------------
+// Read: the tokens [starts[b], starts[b] + rows of b) of each sequence as 16-bit
+// or 32-bit values code * scale. One warp per (touched block, head).
+// ---------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]);
+template <>
+__device__ __forceinline__ void store8<float>(float* p, const float (&x)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+template <>
+__device__ __forceinline__ void store8<__half>(__half* p, const float (&x)[8]) {
+  *reinterpret_cast<uint4*>(p) =
+      make_uint4(from_float2<__half>(x[0], x[1]), from_float2<__half>(x[2], x[3]),
+                 from_float2<__half>(x[4], x[5]), from_float2<__half>(x[6], x[7]));
+}
+template <>
+__device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* p, const float (&x)[8]) {
+  using B = __nv_bfloat16;
+  *reinterpret_cast<uint4*>(p) = make_uint4(from_float2<B>(x[0], x[1]), from_float2<B>(x[2], x[3]),
+                                            from_float2<B>(x[4], x[5]), from_float2<B>(x[6], x[7]));
+}
+
+template <int D, int KIND, typename T>
+__global__ void __launch_bounds__(32 * kAppendWarps) read_kernel(View v, const int32_t* starts,
+                                                                 T* __restrict__ k,
+                                                                 T* __restrict__ val,
+                                                                 int64_t n_warps) {
+  constexpr int R = rec_bytes(D), NC = D / 16;
+  using C = Code<KIND>;
+  __shared__ __align__(128) uint8_t smem[kAppendWarps][(R + 127) / 128 * 128];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int64_t warp = (int64_t)blockIdx.x * kAppendWarps + wid;
+  if (warp >= n_warps) return;
+  const int h = (int)(warp % v.heads);
+  int64_t b, local;
+  find_item(v, warp / v.heads, lane, b, local);
+  const int s = v.slot(b);
+  if (s < 0) return;
+  int64_t r0, r1;
+  v.rows(b, r0, r1);
+  if (r1 == r0) return;
+  const int start = starts ? starts[b] : 0;
+  const int64_t end = start + (r1 - r0);
+  if (start < 0 || end > v.length(s)) {
+    atomicOr(&g_status, kStatusBadIndex);
+    return;
+  }
+  const int64_t blk = start / kBlock + local;
+  if (local < 0 || blk * kBlock >= end) return;
+  const uint8_t* rec = v.record(s, (int)blk, h);
+  if (!rec) return;
+  uint8_t* sm = smem[wid];
+  for (int o = lane * 16; o < R; o += 512)
+    *reinterpret_cast<uint4*>(sm + o) = *reinterpret_cast<const uint4*>(rec + o);
+  __syncwarp();
+  const float ks = *reinterpret_cast<const float*>(sm + 32 * D);
+  const float vs = *reinterpret_cast<const float*>(sm + 32 * D + 4);
+  const int64_t row0 = r0 + blk * kBlock - start;  // output row of the block's token 0
+  const KeyMap km(lane);
+  const ValueMap vm(lane);
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int64_t row = row0 + km.token(i);
+    float x[8];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      float y[4];
+      C::unpack(*reinterpret_cast<const uint32_t*>(sm + km.offset(i, w)), y);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * w + e] = __fmul_rn(y[e], ks);
+    }
+    if (row >= r0 && row < r1) store8<T>(k + (row * v.heads + h) * D + km.channel(i), x);
+  }
+#pragma unroll
+  for (int i = 0; i < NC / 4; ++i) {
+    float x[4][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float y[4];
+      C::unpack(*reinterpret_cast<const uint32_t*>(sm + 16 * D + vm.offset(i, e)), y);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) x[t][e] = __fmul_rn(y[t], vs);
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int64_t row = row0 + vm.token(t);
+      if (row >= r0 && row < r1) store8<T>(val + (row * v.heads + h) * D + vm.channel(i), x[t]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Page operations. table [n_slots, n_cols] (-1: no page), lengths [n_slots],
+// refs [n_pages] live on the device and only kernels change them, so a decode
+// loop needs no host copy of them and no synchronisation.
+// ---------------------------------------------------------------------------
+struct Meta {
+  int32_t* table;
+  int64_t n_slots, n_cols;
+  int32_t* lengths;
+  int32_t* refs;
+  int64_t n_pages;
+  int page_tokens;
+};
+
+constexpr int kPageThreads = 256;
+
+// Whether list[i] is a slot that no earlier place of the list names (block-wide).
+__device__ __forceinline__ bool own_slot(const int32_t* list, int64_t i, int64_t n_slots) {
+  const int s = list[i];
+  bool again = s < 0 || s >= n_slots;
+  for (int64_t j = threadIdx.x; j < i; j += blockDim.x) again |= list[j] == s;
+  return !__syncthreads_or(again);
+}
+
+// One CTA per slot: gives its pages up.
+__global__ void __launch_bounds__(kPageThreads) free_kernel(Meta m, const int32_t* slots,
+                                                            int32_t* status) {
+  if (!own_slot(slots, blockIdx.x, m.n_slots)) {
+    if (threadIdx.x == 0) atomicOr(status, kBadSlot);
+    return;
+  }
+  int32_t* row = m.table + slots[blockIdx.x] * m.n_cols;
+  for (int64_t c = threadIdx.x; c < m.n_cols; c += kPageThreads) {
+    const int p = row[c];
+    if (p >= 0 && p < m.n_pages) atomicSub(&m.refs[p], 1);
+    row[c] = -1;
+  }
+  if (threadIdx.x == 0) m.lengths[slots[blockIdx.x]] = 0;
+}
+
+// One CTA per (src, dst): dst, which has to be empty, shares src's pages.
+__global__ void __launch_bounds__(kPageThreads) fork_kernel(Meta m, const int32_t* src,
+                                                            const int32_t* dst, int64_t n,
+                                                            int32_t* status) {
+  const int from = src[blockIdx.x], to = dst[blockIdx.x];
+  bool bad = !own_slot(dst, blockIdx.x, m.n_slots);
+  bool is_src = from < 0 || from >= m.n_slots;
+  for (int64_t j = threadIdx.x; j < n; j += kPageThreads) is_src |= src[j] == to;
+  bad |= __syncthreads_or(is_src);
+  if (!bad) bad = m.lengths[to] != 0;
+  __syncthreads();  // every thread has read the length before it is written
+  if (bad) {
+    if (threadIdx.x == 0) atomicOr(status, kBadSlot);
+    return;
+  }
+  const int32_t* in = m.table + from * m.n_cols;
+  int32_t* out = m.table + to * m.n_cols;
+  for (int64_t c = threadIdx.x; c < m.n_cols; c += kPageThreads) {
+    const int p = in[c];
+    out[c] = p;
+    if (p >= 0 && p < m.n_pages) atomicAdd(&m.refs[p], 1);
+  }
+  if (threadIdx.x == 0) m.lengths[to] = m.lengths[from];
+}
+
+// Block-wide exclusive scan of one int per thread (1024 threads); total to all.
+__device__ __forceinline__ int block_scan(int x, int* warp_sums, int& total) {
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  int incl = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) warp_sums[wid] = incl;
+  __syncthreads();
+  int before = 0, all = 0;
+  {
+    const int y = lane < nw ? warp_sums[lane] : 0;
+    int z = y;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, z, o);
+      if (lane >= o) z += u;
+    }
+    all = __shfl_sync(0xffffffffu, z, 31);
+    before = __shfl_sync(0xffffffffu, z - y, wid);
+  }
+  __syncthreads();
+  total = all;
+  return before + incl - x;
+}
+
+constexpr int kPlanThreads = 1024;
+
+// Workspace of extend and compact: the number of page moves, then the moves.
+struct Moves {
+  int32_t count, pad[3];
+};
+
+// One CTA: pages for the new tokens of every slot, taken from the free ones in
+// ascending order, slot after slot in the list's order. A slot whose last page
+// is open and shared gets a page of its own for it (to be copied by
+// move_kernel) unless every other holder stands before it in the list. Nothing
+// changes when the call is refused.
+__global__ void __launch_bounds__(kPlanThreads) extend_kernel(Meta m, const int32_t* slots,
+                                                              int64_t n, const int32_t* n_new,
+                                                              int n_new_all, int32_t* status,
+                                                              Moves* moves, int2* list,
+                                                              int32_t* pages) {
+  __shared__ int warp_sums[32];
+  __shared__ int last_page[kMaxSeqs];  // shared open page of slot i, or -1 - i
+  __shared__ int need[kMaxSeqs];       // pages, then its offset; copy flag in `copies`
+  __shared__ uint8_t copies[kMaxSeqs];
+  const int tid = threadIdx.x;
+  int bad = 0;
+  for (int i = tid; i < n; i += kPlanThreads) {
+    const int s = slots[i], add = n_new ? n_new[i] : n_new_all;
+    last_page[i] = -1 - i;
+    need[i] = 0;
+    if (s < 0 || s >= m.n_slots || add < 0) {
+      bad |= kBadSlot;
+      continue;
+    }
+    const int64_t len = m.lengths[s], P = m.page_tokens;
+    if (len < 0 || (len + add + P - 1) / P > m.n_cols) {
+      bad |= kBadSlot;
+      continue;
+    }
+    need[i] = (int)((len + add + P - 1) / P - (len + P - 1) / P);
+    if (add > 0 && len % P) {
+      const int p = m.table[s * m.n_cols + len / P];
+      if (p < 0 || p >= m.n_pages) bad |= kBadSlot;
+      else if (m.refs[p] > 1) last_page[i] = p;
+    }
+  }
+  bad = __syncthreads_or(bad);
+  for (int i = tid; i < n; i += kPlanThreads) {
+    const int s = slots[i], p = last_page[i];
+    int before = 0;
+    for (int j = 0; j < i; ++j) {
+      bad |= slots[j] == s ? kBadSlot : 0;
+      before += last_page[j] == p;
+    }
+    const bool copy = p >= 0 && m.refs[p] - before > 1;
+    copies[i] = copy;
+    need[i] += copy;
+  }
+  bad = __syncthreads_or(bad);
+  if (bad) {
+    if (tid == 0) {
+      atomicOr(status, kBadSlot);
+      moves->count = 0;
+    }
+    return;
+  }
+  int total = 0;
+  for (int64_t i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int64_t i = i0 + tid;
+    int sum;
+    const int at = block_scan(i < n ? need[i] : 0, warp_sums, sum);
+    if (i < n) need[i] = total + at;
+    total += sum;
+  }
+  // the `total` lowest free pages
+  int found = 0;
+  for (int64_t p0 = 0; p0 < m.n_pages && found < total; p0 += kPlanThreads) {
+    const int64_t p = p0 + tid;
+    const bool free = p < m.n_pages && m.refs[p] == 0;
+    int sum;
+    const int at = found + block_scan(free, warp_sums, sum);
+    if (free && at < total) pages[at] = (int)p;
+    found += sum;
+  }
+  if (found < total) {
+    if (tid == 0) {
+      atomicOr(status, kNoPages);
+      moves->count = 0;
+    }
+    return;
+  }
+  __syncthreads();
+  int n_copies = 0;
+  for (int64_t i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int64_t i = i0 + tid;
+    const bool copy = i < n && copies[i];
+    int sum;
+    const int at = n_copies + block_scan(copy, warp_sums, sum);
+    if (copy) list[at] = make_int2(last_page[i], pages[need[i]]);
+    n_copies += sum;
+  }
+  if (tid == 0) moves->count = n_copies;
+  const int lane = tid & 31;
+  for (int64_t i = tid >> 5; i < n; i += kPlanThreads / 32) {
+    const int s = slots[i], add = n_new ? n_new[i] : n_new_all;
+    const int64_t len = m.lengths[s], P = m.page_tokens;
+    const int64_t col = copies[i] ? len / P : (len + P - 1) / P, end = (len + add + P - 1) / P;
+    for (int64_t c = col + lane; c < end; c += 32) {
+      const int p = pages[need[i] + (c - col)];
+      m.table[s * m.n_cols + c] = p;
+      m.refs[p] = 1;
+    }
+    __syncwarp();
+    if (lane == 0) {
+      if (copies[i]) atomicSub(&m.refs[last_page[i]], 1);
+      m.lengths[s] = (int)(len + add);
+    }
+  }
+}
+
+// One CTA: the live pages at or past the number of live pages, in ascending
+// order, move into the free ones below it.
+__global__ void __launch_bounds__(kPlanThreads) compact_kernel(const int32_t* refs,
+                                                               int64_t n_pages, Moves* moves,
+                                                               int2* list, int32_t* new_id,
+                                                               int32_t* n_live) {
+  __shared__ int warp_sums[32];
+  int mine = 0;
+  for (int64_t p = threadIdx.x; p < n_pages; p += kPlanThreads) mine += refs[p] > 0;
+  int live;
+  block_scan(mine, warp_sums, live);
+  int holes = 0, movers = 0;
+  for (int64_t p0 = 0; p0 < n_pages; p0 += kPlanThreads) {
+    const int64_t p = p0 + threadIdx.x;
+    const bool is_live = p < n_pages && refs[p] > 0;
+    const bool hole = p < live && !is_live, mover = p >= live && is_live;
+    int a, c;
+    const int at_hole = holes + block_scan(hole, warp_sums, a);
+    const int at_mover = movers + block_scan(mover, warp_sums, c);
+    if (hole) list[at_hole].y = (int)p;
+    if (mover) list[at_mover].x = (int)p;
+    holes += a;
+    movers += c;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < movers; i += kPlanThreads) new_id[list[i].x] = list[i].y;
+  if (threadIdx.x == 0) {
+    moves->count = movers;
+    *n_live = live;
+  }
+}
+
+// Copies pages src -> dst of every layer as the list says. Bound by HBM.
+__global__ void __launch_bounds__(kPageThreads) move_kernel(const uint8_t* __restrict__ src,
+                                                            uint8_t* __restrict__ dst,
+                                                            int64_t src_layer, int64_t dst_layer,
+                                                            int64_t page_bytes, int n_layers,
+                                                            const Moves* moves, const int2* list) {
+  constexpr int64_t kChunk = kPageThreads * 16 * 4;
+  const int64_t chunks = (page_bytes + kChunk - 1) / kChunk;
+  const int64_t items = (int64_t)moves->count * n_layers * chunks;
+  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    const int64_t chunk = it % chunks, pair = it / chunks;
+    const int2 mv = list[pair / n_layers];
+    const int64_t layer = pair % n_layers;
+    const uint8_t* from = src + layer * src_layer + mv.x * page_bytes;
+    uint8_t* to = dst + layer * dst_layer + mv.y * page_bytes;
+    const int64_t o = chunk * kChunk + threadIdx.x * 16;
+    uint4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (o + i * kPageThreads * 16 < page_bytes)
+        x[i] = *reinterpret_cast<const uint4*>(from + o + i * kPageThreads * 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (o + i * kPageThreads * 16 < page_bytes)
+        *reinterpret_cast<uint4*>(to + o + i * kPageThreads * 16) = x[i];
+  }
+}
+
+// The table and the counts after a compaction.
+__global__ void __launch_bounds__(kPageThreads) renumber_kernel(int32_t* table, int64_t n,
+                                                                int32_t* refs, int64_t n_pages,
+                                                                const Moves* moves,
+                                                                const int2* list,
+                                                                const int32_t* new_id,
+                                                                const int32_t* n_live) {
+  const int live = *n_live, count = moves->count;
+  const int64_t stride = (int64_t)gridDim.x * kPageThreads;
+  const int64_t i0 = (int64_t)blockIdx.x * kPageThreads + threadIdx.x;
+  for (int64_t i = i0; i < n; i += stride) {
+    const int p = table[i];
+    if (p >= live && p < n_pages) table[i] = new_id[p];
+  }
+  for (int64_t i = i0; i < count; i += stride) {
+    refs[list[i].y] = refs[list[i].x];
+    refs[list[i].x] = 0;
+  }
+}
+
+// The move list of a plain copy, with its pairs checked.
+__global__ void __launch_bounds__(kPageThreads) pairs_kernel(const int32_t* src, int64_t n_src,
+                                                             const int32_t* dst, int64_t n_dst,
+                                                             int64_t n, Moves* moves, int2* list) {
+  __shared__ int kept;
+  __shared__ int warp_sums[32];
+  if (threadIdx.x == 0) kept = 0;
+  __syncthreads();
+  for (int64_t i0 = 0; i0 < n; i0 += kPageThreads) {
+    const int64_t i = i0 + threadIdx.x;
+    bool ok = i < n;
+    int a = 0, c = 0;
+    if (ok) {
+      a = src[i];
+      c = dst[i];
+      ok = a >= 0 && a < n_src && c >= 0 && c < n_dst;
+      if (!ok) atomicOr(&g_status, kStatusBadIndex);
+    }
+    int sum;
+    const int at = kept + block_scan(ok, warp_sums, sum);
+    if (ok) list[at] = make_int2(a, c);
+    if (threadIdx.x == 0) kept += sum;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) moves->count = kept;
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+inline int check_view(const char* what, const View& v, int kind, int page_tokens) {
+  if (v.dim != 64 && v.dim != 128) {
+    set_error("%s: head_dim must be 64 or 128 (got %d)", what, v.dim);
+    return KVQ_ERR_UNSUPPORTED;
+  }
+  if (kind != kInt8 && kind != kE4m3) {
+    set_error("%s: kind must be 0 (int8) or 1 (e4m3), got %d", what, kind);
+    return KVQ_ERR_UNSUPPORTED;
+  }
+  if (page_tokens < kBlock || page_tokens > 1024 || page_tokens % kBlock) {
+    set_error("%s: page_tokens must be a multiple of 16 in 16..1024 (got %d)", what, page_tokens);
+    return KVQ_ERR_INVALID;
+  }
+  if (v.n_pages < 1 || v.n_pages > INT32_MAX || v.heads < 1 || v.heads > 1024 || v.n_slots < 1 ||
+      v.n_slots > INT32_MAX || v.n_cols < 1 || v.n_cols > INT32_MAX / page_tokens) {
+    set_error("%s: pool or table of an impossible size (pages %lld, heads %d, table %lld x %lld)",
+              what, (long long)v.n_pages, v.heads, (long long)v.n_slots, (long long)v.n_cols);
+    return KVQ_ERR_INVALID;
+  }
+  if (v.B < 1 || v.B > kMaxSeqs || (!v.slots && v.B > v.n_slots)) {
+    set_error("%s: %lld sequences (1..%d, and no more than the table's rows without slots)", what,
+              (long long)v.B, kMaxSeqs);
+    return KVQ_ERR_INVALID;
+  }
+  if (v.total < 0 || v.total > INT32_MAX || (!v.indptr && v.total % v.B)) {
+    set_error("%s: %lld rows do not divide among %lld sequences", what, (long long)v.total,
+              (long long)v.B);
+    return KVQ_ERR_INVALID;
+  }
+  if (!v.pool || !aligned16(v.pool) || !v.table || !v.lengths) {
+    set_error("%s: the pool must be 16-byte aligned and the table and lengths given", what);
+    return KVQ_ERR_INVALID;
+  }
+  return KVQ_OK;
+}
+
+inline int check_meta(const char* what, const Meta& m) {
+  if (!m.table || !m.refs || m.n_slots < 1 || m.n_slots > INT32_MAX || m.n_cols < 1 ||
+      m.n_pages < 1 || m.n_pages > INT32_MAX || m.page_tokens < kBlock ||
+      m.page_tokens % kBlock || m.n_cols > INT32_MAX / m.page_tokens) {
+    set_error("%s: invalid table (%lld x %lld), counts (%lld pages) or page size %d", what,
+              (long long)m.n_slots, (long long)m.n_cols, (long long)m.n_pages, m.page_tokens);
+    return KVQ_ERR_INVALID;
+  }
+  return KVQ_OK;
+}
+
+inline View make_view(uint8_t* pool, int64_t n_pages, int64_t heads, int64_t dim, int64_t page_tokens,
+                      const int32_t* table, int64_t n_slots, int64_t n_cols,
+                      const int32_t* lengths, const int32_t* slots, const int32_t* indptr,
+                      int64_t B, int64_t total) {
+  View v;
+  v.pool = pool;
+  v.n_pages = n_pages;
+  v.heads = (int)(heads < 0 || heads > INT32_MAX ? 0 : heads);
+  v.dim = (int)(dim < 0 || dim > INT32_MAX ? 0 : dim);
+  v.blocks = (int)(page_tokens / kBlock);
+  v.table = table;
+  v.n_slots = n_slots;
+  v.n_cols = n_cols;
+  v.lengths = lengths;
+  v.slots = slots;
+  v.indptr = indptr;
+  v.B = B;
+  v.total = total;
+  return v;
+}
+
+template <int D, int KIND, typename T>
+static int launch_append(const View& v, const void* k, int64_t k_tok, int64_t k_head,
+                         const void* val, int64_t v_tok, int64_t v_head, cudaStream_t st) {
+  const int64_t warps = block_items(v) * v.heads;
+  const int64_t grid = (warps + kAppendWarps - 1) / kAppendWarps;
+  append_kernel<D, KIND, T><<<(unsigned)grid, 32 * kAppendWarps, 0, st>>>(
+      v, (const T*)k, k_tok, k_head, (const T*)val, v_tok, v_head, warps);
+  return check_launch("paged_append");
+}
+
+template <int D, int KIND, typename T>
+static int launch_read(const View& v, const int32_t* starts, void* k, void* val, cudaStream_t st) {
+  const int64_t warps = block_items(v) * v.heads;
+  const int64_t grid = (warps + kAppendWarps - 1) / kAppendWarps;
+  read_kernel<D, KIND, T><<<(unsigned)grid, 32 * kAppendWarps, 0, st>>>(v, starts, (T*)k, (T*)val,
+                                                                       warps);
+  return check_launch("paged_read");
+}
+
+inline int move_grid() { return 148 * 4; }
+
+inline size_t plan_bytes(int64_t n_pages) {
+  return sizeof(Moves) + (size_t)n_pages * (sizeof(int2) + sizeof(int32_t));
+}
+
+inline int check_pool(const char* what, const uint8_t* pool, int64_t n_layers, int64_t page_bytes) {
+  if (!pool || !aligned16(pool) || n_layers < 1 || n_layers > INT32_MAX || page_bytes < 16 ||
+      page_bytes % 16) {
+    set_error("%s: the pool must be 16-byte aligned with whole records (%lld layers, %lld bytes "
+              "a page)", what, (long long)n_layers, (long long)page_bytes);
+    return KVQ_ERR_INVALID;
+  }
+  return KVQ_OK;
+}
+
+}  // namespace paged
+}  // namespace kvq
+
+extern "C" int kvq_paged_append(const void* k, int64_t k_tok_stride, int64_t k_head_stride,
+                                const void* v, int64_t v_tok_stride, int64_t v_head_stride,
+                                int dtype, uint8_t* pool, int kind, int64_t n_pages,
+                                int64_t n_heads, int64_t head_dim, int64_t page_tokens,
+                                const int32_t* table, int64_t n_slots, int64_t n_cols,
+                                const int32_t* lengths, const int32_t* slots,
+                                const int32_t* indptr, int64_t B, int64_t total, void* stream) {
+  using namespace kvq;
+  using namespace kvq::paged;
+  clear_error();
+  const View w = make_view(pool, n_pages, n_heads, head_dim, page_tokens, table, n_slots, n_cols,
+                           lengths, slots, indptr, B, total);
+  int rc = check_view("paged_append", w, kind, (int)page_tokens);
+  if (rc) return rc;
+  if (dtype != 0 && dtype != 1) {
+    set_error("paged_append: dtype must be 0 (fp16) or 1 (bf16), got %d", dtype);
+    return KVQ_ERR_UNSUPPORTED;
+  }
+  if (total == 0) return KVQ_OK;
+  if (!k || !v || !aligned16(k) || !aligned16(v) || k_tok_stride % 8 || k_head_stride % 8 ||
+      v_tok_stride % 8 || v_head_stride % 8) {
+    set_error("paged_append: k and v rows must be 16-byte aligned (strides multiples of 8)");
+    return KVQ_ERR_INVALID;
+  }
+  if (block_items(w) * w.heads > (int64_t)INT32_MAX * kAppendWarps) {
+    set_error("paged_append: too many rows in one call");
+    return KVQ_ERR_INVALID;
+  }
+  const cudaStream_t st = as_stream(stream);
+#define KVQ_PAGED_APPEND(D, KIND, T) \
+  launch_append<D, KIND, T>(w, k, k_tok_stride, k_head_stride, v, v_tok_stride, v_head_stride, st)
+#define KVQ_PAGED_PICK(D, T) \
+  (kind == kInt8 ? KVQ_PAGED_APPEND(D, kInt8, T) : KVQ_PAGED_APPEND(D, kE4m3, T))
+  if (head_dim == 64)
+    return dtype == 0 ? KVQ_PAGED_PICK(64, __half) : KVQ_PAGED_PICK(64, __nv_bfloat16);
+  return dtype == 0 ? KVQ_PAGED_PICK(128, __half) : KVQ_PAGED_PICK(128, __nv_bfloat16);
+#undef KVQ_PAGED_PICK
+#undef KVQ_PAGED_APPEND
+}
+
+extern "C" int kvq_paged_read(const uint8_t* pool, int kind, int64_t n_pages, int64_t n_heads,
+                              int64_t head_dim, int64_t page_tokens, const int32_t* table,
+                              int64_t n_slots, int64_t n_cols, const int32_t* lengths,
+                              const int32_t* slots, const int32_t* starts, const int32_t* indptr,
+                              int64_t B, int64_t total, void* k_out, void* v_out, int dtype,
+                              void* stream) {
+  using namespace kvq;
+  using namespace kvq::paged;
+  clear_error();
+  const View w = make_view(const_cast<uint8_t*>(pool), n_pages, n_heads, head_dim, page_tokens,
+                           table, n_slots, n_cols, lengths, slots, indptr, B, total);
+  int rc = check_view("paged_read", w, kind, (int)page_tokens);
+  if (rc) return rc;
+  if (dtype < 0 || dtype > 2) {
+    set_error("paged_read: dtype must be 0 (fp16), 1 (bf16) or 2 (fp32), got %d", dtype);
+    return KVQ_ERR_UNSUPPORTED;
+  }
+  if (total == 0) return KVQ_OK;
+  if (!k_out || !v_out || !aligned16(k_out) || !aligned16(v_out)) {
+    set_error("paged_read: the outputs must be 16-byte aligned");
+    return KVQ_ERR_INVALID;
+  }
+  if (block_items(w) * w.heads > (int64_t)INT32_MAX * kAppendWarps) {
+    set_error("paged_read: too many rows in one call");
+    return KVQ_ERR_INVALID;
+  }
+  const cudaStream_t st = as_stream(stream);
+#define KVQ_PAGED_READ(D, T)                                           \
+  (kind == kInt8 ? launch_read<D, kInt8, T>(w, starts, k_out, v_out, st) \
+                 : launch_read<D, kE4m3, T>(w, starts, k_out, v_out, st))
+  if (head_dim == 64)
+    return dtype == 0   ? KVQ_PAGED_READ(64, __half)
+           : dtype == 1 ? KVQ_PAGED_READ(64, __nv_bfloat16)
+                        : KVQ_PAGED_READ(64, float);
+  return dtype == 0   ? KVQ_PAGED_READ(128, __half)
+         : dtype == 1 ? KVQ_PAGED_READ(128, __nv_bfloat16)
+                      : KVQ_PAGED_READ(128, float);
+#undef KVQ_PAGED_READ
+}
+
+extern "C" int kvq_paged_free(int32_t* table, int64_t n_slots, int64_t n_cols, int32_t* lengths,
+                              int32_t* refs, int64_t n_pages, int64_t page_tokens,
+                              const int32_t* slots, int64_t n, int32_t* status, void* stream) {
+  using namespace kvq;
+  using namespace kvq::paged;
+  clear_error();
+  const Meta m{table, n_slots, n_cols, lengths, refs, n_pages, (int)page_tokens};
+  int rc = check_meta("paged_free", m);
+  if (rc) return rc;
+  if (n < 0 || n > kMaxSeqs || !lengths || !status || (n && !slots)) {
+    set_error("paged_free: %lld slots (0..%d), with lengths and status", (long long)n, kMaxSeqs);
+    return KVQ_ERR_INVALID;
+  }
+  if (n == 0) return KVQ_OK;
+  free_kernel<<<(unsigned)n, kPageThreads, 0, as_stream(stream)>>>(m, slots, status);
+  return check_launch("paged_free");
+}
+
+extern "C" int kvq_paged_fork(int32_t* table, int64_t n_slots, int64_t n_cols, int32_t* lengths,
+                              int32_t* refs, int64_t n_pages, int64_t page_tokens,
+                              const int32_t* src, const int32_t* dst, int64_t n, int32_t* status,
+                              void* stream) {
+  using namespace kvq;
+  using namespace kvq::paged;
+  clear_error();
+  const Meta m{table, n_slots, n_cols, lengths, refs, n_pages, (int)page_tokens};
+  int rc = check_meta("paged_fork", m);
+  if (rc) return rc;
+  if (n < 0 || n > kMaxSeqs || !lengths || !status || (n && (!src || !dst))) {
+    set_error("paged_fork: %lld pairs (0..%d), with lengths and status", (long long)n, kMaxSeqs);
+    return KVQ_ERR_INVALID;
+  }
+  if (n == 0) return KVQ_OK;
+  fork_kernel<<<(unsigned)n, kPageThreads, 0, as_stream(stream)>>>(m, src, dst, n, status);
+  return check_launch("paged_fork");
+}
+
+extern "C" size_t kvq_paged_extend_workspace(int64_t n_pages) {
+  return kvq::paged::plan_bytes(n_pages < 0 ? 0 : n_pages);
+}
+
+extern "C" int kvq_paged_extend(uint8_t* pool, int64_t n_layers, int64_t layer_stride,
+                                int64_t page_bytes, int32_t* table, int64_t n_slots,
+                                int64_t n_cols, int32_t* lengths, int32_t* refs, int64_t n_pages,
+                                int64_t page_tokens, const int32_t* slots, int64_t n,
+                                const int32_t* n_new, int64_t n_new_all, int32_t* status,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace kvq;
+  using namespace kvq::paged;
+  clear_error();
+  const Meta m{table, n_slots, n_cols, lengths, refs, n_pages, (int)page_tokens};
+  int rc = check_meta("paged_extend", m);
+  if (!rc) rc = check_pool("paged_extend", pool, n_layers, page_bytes);
+  if (rc) return rc;
+  if (n < 0 || n > kMaxSeqs || !lengths || !status || (n && !slots)) {
+    set_error("paged_extend: %lld slots (0..%d), with lengths and status", (long long)n, kMaxSeqs);
+    return KVQ_ERR_INVALID;
+  }
+  if (!n_new && (n_new_all < 0 || n_new_all > INT32_MAX / 2)) {
+    set_error("paged_extend: %lld new tokens", (long long)n_new_all);
+    return KVQ_ERR_INVALID;
+  }
+  if (layer_stride % 16 || (n_layers > 1 && layer_stride < n_pages * page_bytes)) {
+    set_error("paged_extend: layer stride %lld", (long long)layer_stride);
+    return KVQ_ERR_INVALID;
+  }
+  if (!workspace || !aligned16(workspace) || workspace_bytes < plan_bytes(n_pages)) {
+    set_error("paged_extend: workspace too small or unaligned (%zu < %zu)", workspace_bytes,
+              plan_bytes(n_pages));
+    return KVQ_ERR_INVALID;
+  }
+  if (n == 0) return KVQ_OK;
+  Moves* moves = static_cast<Moves*>(workspace);
+  int2* list = reinterpret_cast<int2*>(moves + 1);
+  int32_t* pages = reinterpret_cast<int32_t*>(list + n_pages);
+  const cudaStream_t st = as_stream(stream);
+  extend_kernel<<<1, kPlanThreads, 0, st>>>(m, slots, n, n_new, (int)n_new_all, status, moves,
+                                            list, pages);
+  rc = check_launch("paged_extend");
+  if (rc) return rc;
+  move_kernel<<<move_grid(), kPageThreads, 0, st>>>(pool, pool, layer_stride, layer_stride,
+                                                    page_bytes, (int)n_layers, moves, list);
+  return check_launch("paged_extend (copy)");
+}
+
+extern "C" int kvq_paged_compact(uint8_t* pool, int64_t n_layers, int64_t layer_stride,
+                                 int64_t page_bytes, int32_t* table, int64_t n_slots,
+                                 int64_t n_cols, int32_t* refs, int64_t n_pages, int32_t* n_live,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace kvq;
+  using namespace kvq::paged;
+  clear_error();
+  const Meta m{table, n_slots, n_cols, nullptr, refs, n_pages, kBlock};
+  int rc = check_meta("paged_compact", m);
+  if (!rc) rc = check_pool("paged_compact", pool, n_layers, page_bytes);
+  if (rc) return rc;
+  if (!n_live) {
+    set_error("paged_compact: n_live is null");
+    return KVQ_ERR_INVALID;
+  }
+  if (layer_stride % 16 || (n_layers > 1 && layer_stride < n_pages * page_bytes)) {
+    set_error("paged_compact: layer stride %lld", (long long)layer_stride);
+    return KVQ_ERR_INVALID;
+  }
+  if (!workspace || !aligned16(workspace) || workspace_bytes < plan_bytes(n_pages)) {
+    set_error("paged_compact: workspace too small or unaligned (%zu < %zu)", workspace_bytes,
+              plan_bytes(n_pages));
+    return KVQ_ERR_INVALID;
+  }
+  Moves* moves = static_cast<Moves*>(workspace);
+  int2* list = reinterpret_cast<int2*>(moves + 1);
+  int32_t* new_id = reinterpret_cast<int32_t*>(list + n_pages);
+  const cudaStream_t st = as_stream(stream);
+  compact_kernel<<<1, kPlanThreads, 0, st>>>(refs, n_pages, moves, list, new_id, n_live);
+  rc = check_launch("paged_compact");
+  if (rc) return rc;
+  move_kernel<<<move_grid(), kPageThreads, 0, st>>>(pool, pool, layer_stride, layer_stride,
+                                                    page_bytes, (int)n_layers, moves, list);
+  rc = check_launch("paged_compact (copy)");
+  if (rc) return rc;
+  renumber_kernel<<<64, kPageThreads, 0, st>>>(table, n_slots * n_cols, refs, n_pages, moves, list,
+                                               new_id, n_live);
+  return check_launch("paged_compact (table)");
+}
+
+extern "C" size_t kvq_paged_copy_workspace(int64_t n) {
+  return sizeof(kvq::paged::Moves) + (n < 0 ? 0 : (size_t)n) * sizeof(int2);
+}
+
+extern "C" int kvq_paged_copy(const uint8_t* src_pool, int64_t src_pages,
+                              int64_t src_layer_stride, uint8_t* dst_pool, int64_t dst_pages,
+                              int64_t dst_layer_stride, int64_t n_layers, int64_t page_bytes,
+                              const int32_t* src, const int32_t* dst, int64_t n, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  using namespace kvq;
+  using namespace kvq::paged;
+  clear_error();
+  int rc = check_pool("paged_copy", src_pool, n_layers, page_bytes);
+  if (!rc) rc = check_pool("paged_copy", dst_pool, n_layers, page_bytes);
+  if (rc) return rc;
+  if (n < 0 || n > INT32_MAX || (n && (!src || !dst)) || src_pages < 1 || dst_pages < 1 ||
+      src_pages > INT32_MAX || dst_pages > INT32_MAX || src_layer_stride % 16 ||
+      dst_layer_stride % 16) {
+    set_error("paged_copy: invalid pairs (%lld), pools (%lld, %lld pages) or strides",
+              (long long)n, (long long)src_pages, (long long)dst_pages);
+    return KVQ_ERR_INVALID;
+  }
+  if (n == 0) return KVQ_OK;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < kvq_paged_copy_workspace(n)) {
+    set_error("paged_copy: workspace too small or unaligned (%zu < %zu)", workspace_bytes,
+              kvq_paged_copy_workspace(n));
+    return KVQ_ERR_INVALID;
+  }
+  Moves* moves = static_cast<Moves*>(workspace);
+  int2* list = reinterpret_cast<int2*>(moves + 1);
+  const cudaStream_t st = as_stream(stream);
+  pairs_kernel<<<1, kPageThreads, 0, st>>>(src, src_pages, dst, dst_pages, n, moves, list);
+  rc = check_launch("paged_copy");
+  if (rc) return rc;
+  move_kernel<<<move_grid(), kPageThreads, 0, st>>>(src_pool, dst_pool, src_layer_stride,
+                                                    dst_layer_stride, page_bytes, (int)n_layers,
+                                                    moves, list);
+  return check_launch("paged_copy (pages)");
+}

@@ -1,0 +1,570 @@
+// Attention over the paged 8-bit KV cache (records and pages: kvq_paged.cuh).
+// Part of the kvq_lib.cu unity build.
+//
+// For query row i of a sequence (its new tokens are its last n tokens, row i at
+// position len - n + i) and KV head h:
+//   t_j = (q . kcode_j) ks_b scale log2(e)            (b the block of token j)
+//   p_j = 2^(t_j - m), out = sum_j p_j vs_b vcode_j / sum_j p_j
+// over the tokens j <= position, j > position - window. The value scale joins
+// the exponent: w_j = 2^(t_j + log2 vs_b - m2) <= 1 with m2 the running maximum
+// of the exponents, so that the fp16 weights of the second product are relative
+// to the largest contribution whatever the blocks' scales are; the softmax sum
+// is sum_j w_j / vs_b in the same reference, out = O / that. Codes are exact in
+// fp16 (8 bits), fp16 queries too, and bf16 queries once a row is scaled by a
+// power of two; products and sums are fp32. The only roundings to fewer bits
+// are w_j (fp16, relative 2^-12, or 2^-25 of the largest) and the output.
+#pragma once
+#include "kvq_paged.cuh"
+
+namespace kvq {
+namespace paged {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct AttnArgs {
+  View v;
+  const void* q;
+  int64_t q_tok, q_head;  // strides in elements
+  int group, max_new, window;
+  float scale_log2;       // softmax scale * log2(e)
+  void* out;              // [total, heads * group, D]
+  float2* ml;             // [total, heads * group] or null: (max, 1 / sum) of each row
+  float* part;            // workspace
+  int n_workers;
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// D (16 x 8, fp32) += A (16 x 16, fp16) B (16 x 8, fp16).
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// The four codes of a word as two fp16 pairs (exact).
+template <int KIND>
+__device__ __forceinline__ void code_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (KIND == kInt8) {
+    // bytes u = code + 128 under the high byte 0x64 are the fp16 numbers 1024 + u
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    uint32_t a = prmt(w, 0x64646464u, 0x4140), b = prmt(w, 0x64646464u, 0x4342);
+    __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), bias);
+    __half2 y = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
+    lo = *reinterpret_cast<uint32_t*>(&x);
+    hi = *reinterpret_cast<uint32_t*>(&y);
+  } else {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+  }
+}
+
+// What one call sees of sequence b. A row group is R = 8 * NT query rows (token,
+// query head of the KV head's group), row r being token r / group.
+struct Seq {
+  int slot, len, n, lo_blk, n_blk, groups;
+  int64_t r0;
+};
+__device__ __forceinline__ Seq load_seq(const AttnArgs& a, int64_t b, int R) {
+  Seq s;
+  int64_t r1;
+  a.v.rows(b, s.r0, r1);
+  s.n = (int)(r1 - s.r0);
+  if (s.n > a.max_new) {
+    atomicOr(&g_status, kStatusBadIndex);
+    s.n = 0;
+  }
+  s.slot = a.v.slot(b);
+  s.len = s.slot < 0 ? 0 : a.v.length(s.slot);
+  const int lo = a.window > 0 ? max(0, s.len - s.n - a.window + 1) : 0;
+  s.lo_blk = lo / kBlock;
+  // an empty sequence still has a (wholly masked) block, which writes its rows
+  s.n_blk = max(1, (s.len + kBlock - 1) / kBlock - s.lo_blk);
+  s.groups = (int)(((int64_t)s.n * a.group + R - 1) / R);
+  if (s.n == 0) s.n_blk = 0;
+  return s;
+}
+
+// Work is a flat sequence of 16-token blocks over (sequence, head, row group),
+// and worker w of W takes an equal share of it, whatever the lengths are. pre[b]
+// = blocks of the sequences before b, per head. Block-wide; pre has B + 1 places.
+template <int THREADS>
+__device__ __forceinline__ int64_t block_prefix(const AttnArgs& a, int R, int64_t* pre,
+                                                int64_t* sums) {
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  int64_t base = 0;
+  for (int64_t b0 = 0; b0 < a.v.B; b0 += THREADS) {
+    const int64_t b = b0 + threadIdx.x;
+    int64_t x = 0;
+    if (b < a.v.B) {
+      const Seq s = load_seq(a, b, R);
+      x = (int64_t)s.n_blk * s.groups;
+    }
+    int64_t incl = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) sums[wid] = incl;
+    __syncthreads();
+    int64_t before = base;
+    for (int i = 0; i < THREADS / 32; ++i) {
+      if (i < wid) before += sums[i];
+      base += sums[i];
+    }
+    if (b < a.v.B) pre[b] = before + incl - x;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) pre[a.v.B] = base;
+  __syncthreads();
+  return base * a.v.heads;
+}
+
+// Workers that a call of `total` blocks keeps busy.
+__device__ __forceinline__ int64_t workers_of(const AttnArgs& a, int64_t total) {
+  return max((int64_t)1, min((int64_t)a.n_workers, total));
+}
+
+__host__ __device__ constexpr int part_floats(int D, int NT) { return 8 * NT * (D + 4); }
+
+// One row group's running state in a warp. Scores are S^T (tokens x rows): lane
+// (g, c) = (lane / 4, lane % 4) holds tokens g, g + 8 of rows 2c, 2c + 1 of each
+// 8-row tile; outputs are O^T (channels x rows) in the same layout.
+template <int D, int NT>
+struct State {
+  float o[D / 16][NT][4];
+  float m[NT][2], m2[NT][2], l[NT][2];
+  __device__ void clear() {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+        o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.f;
+      m[t][0] = m[t][1] = m2[t][0] = m2[t][1] = -INFINITY;
+      l[t][0] = l[t][1] = 0.f;
+    }
+  }
+};
+
+// Query fragments of a row group: rows in the B operand's columns.
+template <int D, int NT, typename T>
+__device__ __forceinline__ void load_q(const AttnArgs& a, const Seq& s, int h, int row0, int lane,
+                                       uint32_t (&qf)[D / 16][NT][2], float (&qs)[NT][2]) {
+  const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int r = row0 + 8 * t + g;
+    const bool valid = r < s.n * a.group;
+    const T* p = (const T*)a.q + (s.r0 + r / a.group) * a.q_tok +
+                 (int64_t)(h * a.group + r % a.group) * a.q_head;
+    float f = 1.f, inv = 1.f;
+    uint2 w[D / 16];
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j)
+      w[j] = valid ? *reinterpret_cast<const uint2*>(p + 16 * j + 4 * c) : make_uint2(0, 0);
+    if constexpr (!std::is_same<T, __half>::value) {
+      float mx = 0.f;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        const float2 x = to_float2<T>(w[j].x), y = to_float2<T>(w[j].y);
+        mx = fmaxf(fmaxf(mx, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(y.x), fabsf(y.y)));
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      // the row's largest value to [2^14, 2^15)
+      const int e = max(-100, (int)((__float_as_uint(mx) >> 23) & 255) - 127);
+      if (mx > 0.f && mx < INFINITY) {
+        f = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+        inv = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+      }
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        const float2 x = to_float2<T>(w[j].x), y = to_float2<T>(w[j].y);
+        w[j] = make_uint2(half2_bits(x.x * f, x.y * f), half2_bits(y.x * f, y.y * f));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      qf[j][t][0] = w[j].x;
+      qf[j][t][1] = w[j].y;
+    }
+    // the scores' factor, from the lanes of rows 2c and 2c + 1
+    qs[t][0] = a.scale_log2 * __shfl_sync(0xffffffffu, inv, 8 * c);
+    qs[t][1] = a.scale_log2 * __shfl_sync(0xffffffffu, inv, 8 * c + 4);
+  }
+}
+
+// One block of 16 tokens into the state. kc, vc: the lane's code words; MASK:
+// some token of the block is hidden from some row, or past the end.
+template <int D, int KIND, int NT, bool MASK>
+__device__ __forceinline__ void block_step(State<D, NT>& st, const uint4 (&kc)[D / 32],
+                                           const uint4 (&vc)[D / 32], float ks, float vs,
+                                           const uint32_t (&qf)[D / 16][NT][2],
+                                           const float (&qs)[NT][2], int t0, int len,
+                                           const int (&lo)[NT][2], const int (&hi)[NT][2],
+                                           int lane) {
+  const int g = lane >> 2, c = lane & 3;
+  float s[NT][2][4];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[t][0][e] = s[t][1][e] = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    const uint32_t w[4] = {kc[i].x, kc[i].y, kc[i].z, kc[i].w};
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj) {
+      uint32_t a0, a1, a2, a3;
+      code_halves<KIND>(w[2 * jj], a0, a2);
+      code_halves<KIND>(w[2 * jj + 1], a1, a3);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        mma16816(s[t][jj], a0, a1, a2, a3, qf[2 * i + jj][t][0], qf[2 * i + jj][t][1]);
+    }
+  }
+  const float lv = __log2f(vs), ivs = __fdividef(1.f, vs);
+  uint32_t pb[NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    float x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[e] = (s[t][0][e] + s[t][1][e]) * (ks * qs[t][e & 1]);
+      if (MASK) {
+        const int j = t0 + g + 8 * (e >> 1);
+        if (j > hi[t][e & 1] || j < lo[t][e & 1]) x[e] = -INFINITY;
+      }
+    }
+    bool grew = false;
+    float alpha[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float bm = fmaxf(x[r], x[r + 2]);
+      bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 4));
+      bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 8));
+      bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 16));
+      st.m[t][r] = fmaxf(st.m[t][r], bm);
+      const float was = st.m2[t][r], now = fmaxf(was, bm + lv);
+      grew |= now > was;
+      const float ref = now == -INFINITY ? 0.f : now;
+      alpha[r] = exp2_approx(was - ref);
+      st.m2[t][r] = now;
+      x[r] = exp2_approx(x[r] + (lv - ref));
+      x[r + 2] = exp2_approx(x[r + 2] + (lv - ref));
+    }
+    if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        st.o[i][t][0] *= alpha[0];
+        st.o[i][t][1] *= alpha[1];
+        st.o[i][t][2] *= alpha[0];
+        st.o[i][t][3] *= alpha[1];
+      }
+      st.l[t][0] *= alpha[0];
+      st.l[t][1] *= alpha[1];
+    }
+    st.l[t][0] = fmaf(x[0] + x[2], ivs, st.l[t][0]);
+    st.l[t][1] = fmaf(x[1] + x[3], ivs, st.l[t][1]);
+    pb[t][0] = transpose8x8(half2_bits(x[0], x[1]));
+    pb[t][1] = transpose8x8(half2_bits(x[2], x[3]));
+  }
+  uint32_t vmask = 0xffffffffu;
+  if (MASK && KIND == kE4m3) {
+    // places past the end may hold anything, and 0 times a NaN code is a NaN
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (t0 + 2 * c + (e & 1) + 8 * (e >> 1) >= len) vmask &= ~(0xffu << (8 * e));
+  }
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    const uint32_t w[4] = {vc[i].x, vc[i].y, vc[i].z, vc[i].w};
+#pragma unroll
+    for (int mm = 0; mm < 2; ++mm) {
+      uint32_t a0, a1, a2, a3;
+      code_halves<KIND>(MASK ? w[2 * mm] & vmask : w[2 * mm], a0, a2);
+      code_halves<KIND>(MASK ? w[2 * mm + 1] & vmask : w[2 * mm + 1], a1, a3);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        mma16816(st.o[2 * i + mm][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) {
+  return __float2bfloat16_rn(x);
+}
+
+// (max, 1 / sum) of a row in natural units; a row that sees nothing has (-inf, inf).
+__device__ __forceinline__ float2 row_stats(float m, float m2, float l) {
+  if (l == 0.f) return make_float2(-INFINITY, INFINITY);
+  return make_float2(m * kLn2, __fdiv_rn(1.f, l * exp2f(m2 - m)));
+}
+
+constexpr int kAttnWarps = 4;
+constexpr int kAttnCtasPerSm = 4;
+constexpr int kSms = 148;
+
+template <int D, int KIND, int NT, typename T>
+__global__ void __launch_bounds__(32 * kAttnWarps) attend_kernel(AttnArgs a) {
+  constexpr int R = 8 * NT;
+  extern __shared__ int64_t pre[];  // B + 1, then the scan's warp sums
+  const int lane = threadIdx.x & 31;
+  const int64_t total = block_prefix<32 * kAttnWarps>(a, R, pre, pre + a.v.B + 1);
+  const int64_t W = workers_of(a, total);
+  const int64_t w = (int64_t)blockIdx.x * kAttnWarps + (threadIdx.x >> 5);
+  if (w >= W || total == 0) return;
+  int64_t x = total * w / W;
+  const int64_t end = total * (w + 1) / W;
+  const int g = lane >> 2, c = lane & 3;
+  while (x < end) {
+    int64_t b = 0, hi_b = a.v.B;  // largest b with pre[b] * heads <= x
+    while (hi_b - b > 1) {
+      const int64_t mid = (b + hi_b) >> 1;
+      if (pre[mid] * a.v.heads <= x) b = mid;
+      else hi_b = mid;
+    }
+    const Seq s = load_seq(a, b, R);
+    const int64_t rem = x - pre[b] * a.v.heads;
+    const int unit = (int)(rem / s.n_blk), blk0 = (int)(rem % s.n_blk);
+    const int n = (int)min((int64_t)(s.n_blk - blk0), end - x);
+    const int h = unit / s.groups, row0 = unit % s.groups * R;
+    x += n;
+
+    uint32_t qf[D / 16][NT][2];
+    float qs[NT][2];
+    load_q<D, NT, T>(a, s, h, row0, lane, qf, qs);
+    int lo[NT][2], hi[NT][2];
+    const int rows = s.n * a.group;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int row = row0 + 8 * t + 2 * c + r, pos = s.len - s.n + row / a.group;
+        hi[t][r] = row < rows ? pos : -1;
+        lo[t][r] = a.window > 0 ? pos - a.window + 1 : 0;
+      }
+    // tokens [see_lo, see_hi] are visible to every row of the group
+    const int see_hi = s.len - s.n + row0 / a.group;
+    const int last = s.len - s.n + (min(row0 + R, rows) - 1) / a.group;
+    const int see_lo = a.window > 0 ? last - a.window + 1 : 0;
+    State<D, NT> st;
+    st.clear();
+    for (int i = 0; i < n; ++i) {
+      const int blk = s.lo_blk + blk0 + i, t0 = blk * kBlock;
+      if (t0 >= s.len) continue;
+      const uint8_t* rec = a.v.record(s.slot, blk, h);
+      if (!rec) continue;
+      uint4 kc[D / 32], vc[D / 32];
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) {
+        kc[k] = *reinterpret_cast<const uint4*>(rec + 512 * k + 16 * lane);
+        vc[k] = *reinterpret_cast<const uint4*>(rec + 16 * D + 512 * k + 16 * lane);
+      }
+      const float2 sc = *reinterpret_cast<const float2*>(rec + 32 * D);
+      if (t0 >= see_lo && t0 + kBlock - 1 <= see_hi)
+        block_step<D, KIND, NT, false>(st, kc, vc, sc.x, sc.y, qf, qs, t0, s.len, lo, hi, lane);
+      else
+        block_step<D, KIND, NT, true>(st, kc, vc, sc.x, sc.y, qf, qs, t0, s.len, lo, hi, lane);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float l = st.l[t][r];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        st.l[t][r] = l;
+      }
+    if (n == s.n_blk) {  // the whole unit: its rows are done
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int row = row0 + 8 * t + 2 * c + r;
+          if (row >= rows) continue;
+          const int64_t at = (s.r0 + row / a.group) * ((int64_t)a.v.heads * a.group) +
+                             h * a.group + row % a.group;
+          const float inv = st.l[t][r] == 0.f ? 0.f : __fdiv_rn(1.f, st.l[t][r]);
+          T* out = (T*)a.out + at * D;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            out[16 * i + g] = from_float<T>(st.o[i][t][r] * inv);
+            out[16 * i + 8 + g] = from_float<T>(st.o[i][t][r + 2] * inv);
+          }
+          if (a.ml && g == 0) a.ml[at] = row_stats(st.m[t][r], st.m2[t][r], st.l[t][r]);
+        }
+    } else {
+      float* p = a.part + (2 * w + (blk0 == 0)) * part_floats(D, NT);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int row = 8 * t + 2 * c + r;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            p[row * D + 16 * i + g] = st.o[i][t][r];
+            p[row * D + 16 * i + 8 + g] = st.o[i][t][r + 2];
+          }
+          if (g == 0)
+            *reinterpret_cast<float4*>(p + R * D + 4 * row) =
+                make_float4(st.m2[t][r], st.l[t][r], st.m[t][r], 0.f);
+        }
+    }
+  }
+}
+
+// Joins the pieces of the units that several workers share, in the workers'
+// order: one CTA of D threads per (unit, row).
+template <int D, int NT, typename T>
+__global__ void __launch_bounds__(D) attend_join_kernel(AttnArgs a) {
+  constexpr int R = 8 * NT;
+  extern __shared__ int64_t pre[];
+  const int64_t total = block_prefix<D>(a, R, pre, pre + a.v.B + 1);
+  const int64_t W = workers_of(a, total);
+  const int64_t b = blockIdx.y;
+  const Seq s = load_seq(a, b, R);
+  const int unit = blockIdx.x / R, r = blockIdx.x % R;
+  if (total == 0 || unit >= s.groups * a.v.heads) return;
+  const int h = unit / s.groups, row = unit % s.groups * R + r;
+  if (row >= s.n * a.group) return;
+  const int64_t x0 = pre[b] * a.v.heads + (int64_t)unit * s.n_blk, x1 = x0 + s.n_blk;
+  // worker w holds the blocks [total w / W, total (w + 1) / W)
+  const int64_t w0 = ((x0 + 1) * W - 1) / total, w1 = (x1 * W - 1) / total;
+  if (w0 == w1) return;
+  const int d = threadIdx.x;
+  float m = -INFINITY, m2 = -INFINITY, l = 0.f, o = 0.f;
+  for (int64_t w = w0; w <= w1; ++w) {
+    const bool from_start = w == w0;
+    const float* p = a.part + (2 * w + from_start) * part_floats(D, NT);
+    const float4 q = *reinterpret_cast<const float4*>(p + R * D + 4 * r);
+    const float now = fmaxf(m2, q.x), ref = now == -INFINITY ? 0.f : now;
+    const float f0 = exp2_approx(m2 - ref), f1 = exp2_approx(q.x - ref);
+    o = o * f0 + p[r * D + d] * f1;
+    l = l * f0 + q.y * f1;
+    m = fmaxf(m, q.z);
+    m2 = now;
+  }
+  const int64_t at = (s.r0 + row / a.group) * ((int64_t)a.v.heads * a.group) + h * a.group +
+                     row % a.group;
+  ((T*)a.out)[at * D + d] = from_float<T>(l == 0.f ? 0.f : o * __fdiv_rn(1.f, l));
+  if (a.ml && d == 0) a.ml[at] = row_stats(m, m2, l);
+}
+
+// Rows of a call's largest sequence: one 8-row tile where that is enough.
+inline int row_tiles(int64_t max_new, int64_t group) { return max_new * group <= 8 ? 1 : 2; }
+
+inline size_t attention_bytes(int64_t D, int64_t max_new, int64_t group) {
+  const int NT = row_tiles(max_new, group);
+  return (size_t)2 * kSms * kAttnCtasPerSm * kAttnWarps * part_floats((int)D, NT) * sizeof(float);
+}
+
+template <int D, int KIND, int NT, typename T>
+static int launch_attend(AttnArgs a, cudaStream_t st) {
+  const int smem = (int)((a.v.B + 1 + 32) * sizeof(int64_t));
+  const int64_t groups = ((int64_t)a.max_new * a.group + 8 * NT - 1) / (8 * NT);
+  a.n_workers = kSms * kAttnCtasPerSm * kAttnWarps;
+  attend_kernel<D, KIND, NT, T><<<kSms * kAttnCtasPerSm, 32 * kAttnWarps, smem, st>>>(a);
+  int rc = check_launch("paged_attention");
+  if (rc) return rc;
+  const dim3 grid((unsigned)(groups * a.v.heads * 8 * NT), (unsigned)a.v.B);
+  attend_join_kernel<D, NT, T><<<grid, D, smem, st>>>(a);
+  return check_launch("paged_attention (join)");
+}
+
+}  // namespace paged
+}  // namespace kvq
+
+extern "C" size_t kvq_paged_attention_workspace(int64_t head_dim, int64_t max_new, int64_t group) {
+  if (head_dim < 0 || head_dim > 128 || max_new < 0 || group < 0) return 0;
+  return kvq::paged::attention_bytes(head_dim, max_new, group);
+}
+
+extern "C" int kvq_paged_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                                   int dtype, int64_t group, const uint8_t* pool, int kind,
+                                   int64_t n_pages, int64_t n_heads, int64_t head_dim,
+                                   int64_t page_tokens, const int32_t* table, int64_t n_slots,
+                                   int64_t n_cols, const int32_t* lengths, const int32_t* slots,
+                                   const int32_t* indptr, int64_t B, int64_t total,
+                                   int64_t max_new, float scale, int64_t window, void* out,
+                                   float* ml_out, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  using namespace kvq;
+  using namespace kvq::paged;
+  clear_error();
+  AttnArgs a;
+  a.v = make_view(const_cast<uint8_t*>(pool), n_pages, n_heads, head_dim, page_tokens, table,
+                  n_slots, n_cols, lengths, slots, indptr, B, total);
+  int rc = check_view("paged_attention", a.v, kind, (int)page_tokens);
+  if (rc) return rc;
+  if (dtype != 0 && dtype != 1) {
+    set_error("paged_attention: dtype must be 0 (fp16) or 1 (bf16), got %d", dtype);
+    return KVQ_ERR_UNSUPPORTED;
+  }
+  if (group < 1 || group > 64 || n_heads * group > 4096) {
+    set_error("paged_attention: %lld query heads per KV head (1..64) of %lld", (long long)group,
+              (long long)n_heads);
+    return KVQ_ERR_UNSUPPORTED;
+  }
+  if (max_new < 0 || max_new > 65536 || (!indptr && max_new < total / B) || window < 0 ||
+      window > INT32_MAX) {
+    set_error("paged_attention: max_new %lld (0..65536, at least the rows a sequence) or window "
+              "%lld", (long long)max_new, (long long)window);
+    return KVQ_ERR_INVALID;
+  }
+  if (total == 0 || max_new == 0) return KVQ_OK;
+  if (!q || !out || !aligned16(q) || q_tok_stride % 8 || q_head_stride % 8 ||
+      (reinterpret_cast<uintptr_t>(out) & 15) || (reinterpret_cast<uintptr_t>(ml_out) & 7)) {
+    set_error("paged_attention: q rows and out must be 16-byte aligned (strides multiples of 8), "
+              "ml_out 8-byte aligned");
+    return KVQ_ERR_INVALID;
+  }
+  const size_t need = attention_bytes(head_dim, max_new, group);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < need) {
+    set_error("paged_attention: workspace too small or unaligned (%zu < %zu)", workspace_bytes,
+              need);
+    return KVQ_ERR_INVALID;
+  }
+  a.q = q;
+  a.q_tok = q_tok_stride;
+  a.q_head = q_head_stride;
+  a.group = (int)group;
+  a.max_new = (int)max_new;
+  a.window = (int)window;
+  a.scale_log2 = scale * kLog2e;
+  a.out = out;
+  a.ml = reinterpret_cast<float2*>(ml_out);
+  a.part = static_cast<float*>(workspace);
+  const cudaStream_t st = as_stream(stream);
+  const int NT = row_tiles(max_new, group);
+#define KVQ_ATTEND3(D, KIND, T) \
+  (NT == 1 ? launch_attend<D, KIND, 1, T>(a, st) : launch_attend<D, KIND, 2, T>(a, st))
+#define KVQ_ATTEND2(D, T) (kind == kInt8 ? KVQ_ATTEND3(D, kInt8, T) : KVQ_ATTEND3(D, kE4m3, T))
+  if (head_dim == 64)
+    return dtype == 0 ? KVQ_ATTEND2(64, __half) : KVQ_ATTEND2(64, __nv_bfloat16);
+  return dtype == 0 ? KVQ_ATTEND2(128, __half) : KVQ_ATTEND2(128, __nv_bfloat16);
+#undef KVQ_ATTEND2
+#undef KVQ_ATTEND3
+}

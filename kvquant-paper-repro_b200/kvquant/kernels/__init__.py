@@ -5,7 +5,9 @@ from .cuda_ops import get_cuda_ops, cuda_available
 from .decode import (quantize_keys, quantize_values, qk_scores, qk_scores_stats, softmax,
                      pv_out, pv_out_scores, decode_attention, make_appendable, append_keys,
                      append_values, key_outlier_thresholds, decode_attention_shard,
-                     merge_shards, set_decode_kernels)
+                     merge_shards, set_decode_kernels, DecodeWorkspace)
+from .paged import (paged_append, paged_read, paged_attention, paged_free, paged_fork,
+                    paged_extend, paged_compact, paged_copy)
 
 __all__ = [
     "apply_rope_elementwise",
@@ -31,4 +33,13 @@ __all__ = [
     "decode_attention_shard",
     "merge_shards",
     "set_decode_kernels",
+    "DecodeWorkspace",
+    "paged_append",
+    "paged_read",
+    "paged_attention",
+    "paged_free",
+    "paged_fork",
+    "paged_extend",
+    "paged_compact",
+    "paged_copy",
 ]

@@ -101,6 +101,29 @@ _SIGNATURES = {
                                       _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_int, _c_p,
                                       _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_p,
                                       _c_p, _c_p, _c_size, _c_p]),
+    "kvq_paged_append": (_c_int, [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_int, _c_p, _c_int,
+                                  _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p,
+                                  _c_p, _c_i64, _c_i64, _c_p]),
+    "kvq_paged_read": (_c_int, [_c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
+                                _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_int, _c_p]),
+    "kvq_paged_attention_workspace": (_c_size, [_c_i64, _c_i64, _c_i64]),
+    "kvq_paged_attention": (_c_int, [_c_p, _c_i64, _c_i64, _c_int, _c_i64, _c_p, _c_int, _c_i64,
+                                     _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p,
+                                     _c_p, _c_i64, _c_i64, _c_i64, _c_flt, _c_i64, _c_p, _c_p,
+                                     _c_p, _c_size, _c_p]),
+    "kvq_paged_free": (_c_int, [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_i64,
+                                _c_p, _c_p]),
+    "kvq_paged_fork": (_c_int, [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p,
+                                _c_i64, _c_p, _c_p]),
+    "kvq_paged_extend_workspace": (_c_size, [_c_i64]),
+    "kvq_paged_extend": (_c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p,
+                                  _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_size,
+                                  _c_p]),
+    "kvq_paged_compact": (_c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p,
+                                   _c_i64, _c_p, _c_p, _c_size, _c_p]),
+    "kvq_paged_copy_workspace": (_c_size, [_c_i64]),
+    "kvq_paged_copy": (_c_int, [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p,
+                                _c_p, _c_i64, _c_p, _c_size, _c_p]),
 }
 
 _lock = threading.Lock()
