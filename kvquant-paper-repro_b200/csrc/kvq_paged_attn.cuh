@@ -322,36 +322,151 @@ __device__ __forceinline__ float2 row_stats(float m, float m2, float l) {
   return make_float2(m * kLn2, __fdiv_rn(1.f, l * exp2f(m2 - m)));
 }
 
-constexpr int kAttnWarps = 4;
-constexpr int kAttnCtasPerSm = 4;
+// Programmatic dependent launch: a kernel launched with that attribute may start
+// while the one before it in the stream still runs, and sees its writes only after
+// wait_previous(); let_next_start() allows the next such launch to begin.
+__device__ __forceinline__ void wait_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+constexpr int kAttnWarps = 8;  // consumers; one more warp feeds them
+constexpr int kAttnThreads = 32 * (kAttnWarps + 1);
 constexpr int kSms = 148;
 
-template <int D, int KIND, int NT, typename T>
-__global__ void __launch_bounds__(32 * kAttnWarps) attend_kernel(AttnArgs a) {
-  constexpr int R = 8 * NT;
-  extern __shared__ int64_t pre[];  // B + 1, then the scan's warp sums
-  const int lane = threadIdx.x & 31;
-  const int64_t total = block_prefix<32 * kAttnWarps>(a, R, pre, pre + a.v.B + 1);
-  const int64_t W = workers_of(a, total);
-  const int64_t w = (int64_t)blockIdx.x * kAttnWarps + (threadIdx.x >> 5);
-  if (w >= W || total == 0) return;
-  int64_t x = total * w / W;
-  const int64_t end = total * (w + 1) / W;
-  const int g = lane >> 2, c = lane & 3;
-  while (x < end) {
-    int64_t b = 0, hi_b = a.v.B;  // largest b with pre[b] * heads <= x
-    while (hi_b - b > 1) {
-      const int64_t mid = (b + hi_b) >> 1;
-      if (pre[mid] * a.v.heads <= x) b = mid;
-      else hi_b = mid;
-    }
-    const Seq s = load_seq(a, b, R);
-    const int64_t rem = x - pre[b] * a.v.heads;
-    const int unit = (int)(rem / s.n_blk), blk0 = (int)(rem % s.n_blk);
-    const int n = (int)min((int64_t)(s.n_blk - blk0), end - x);
-    const int h = unit / s.groups, row0 = unit % s.groups * R;
-    x += n;
+template <int D>
+struct Ring {
+  // 6 (D = 128) or 11 records per warp, up to 197 KB in flight per SM; the rest of
+  // shared memory holds the prefix of up to kMaxSeqs sequences
+  static constexpr int kStages = D == 128 ? 6 : 11;
+  static constexpr int kBytes = kAttnWarps * kStages * rec_bytes(D);
+};
 
+template <int D>
+struct AttnSmem {
+  alignas(128) uint8_t ring[kAttnWarps][Ring<D>::kStages][rec_bytes(D)];
+  uint64_t full[kAttnWarps][Ring<D>::kStages], empty[kAttnWarps][Ring<D>::kStages];
+  int skip[kAttnWarps][Ring<D>::kStages];
+  int abort;
+  int64_t sums[32];
+  int64_t pre[1];  // B + 1
+};
+
+// Where a worker stands in its share of the blocks.
+struct Cursor {
+  int64_t x, end;
+  int64_t b;
+  Seq s;
+  int unit, blk0, n;
+  // The next piece (blocks of one unit); false when the share is done.
+  __device__ bool next(const AttnArgs& a, int R, const int64_t* pre) {
+    if (x >= end) return false;
+    int64_t lo = 0, hi = a.v.B;  // largest b with pre[b] * heads <= x
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (pre[mid] * a.v.heads <= x) lo = mid;
+      else hi = mid;
+    }
+    b = lo;
+    s = load_seq(a, b, R);
+    const int64_t rem = x - pre[b] * a.v.heads;
+    unit = (int)(rem / s.n_blk);
+    blk0 = (int)(rem % s.n_blk);
+    n = (int)min((int64_t)(s.n_blk - blk0), end - x);
+    x += n;
+    return true;
+  }
+};
+
+// One CTA per SM. Every consumer warp works through its own share of the blocks
+// with its own ring of records, so no warp waits for another one; a lane of the
+// ninth warp keeps each ring full: one bulk copy per record, ring after ring
+// across the ends of units. 8 warps hide the ~500 cycles a block takes a warp
+// (HBM delivers one per ~180 cycles and SM).
+template <int D, int KIND, int NT, typename T>
+__global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
+  constexpr int R = 8 * NT, S = Ring<D>::kStages;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  AttnSmem<D>& sm = *reinterpret_cast<AttnSmem<D>*>(smem_raw);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x < kAttnWarps * S) {
+    sm100::mbar_init(&sm.full[0][0] + threadIdx.x, 1);
+    sm100::mbar_init(&sm.empty[0][0] + threadIdx.x, 1);
+  }
+  if (threadIdx.x == 0) sm.abort = 0;
+  sm100::fence_mbar_init();
+  wait_previous();
+  let_next_start();
+  const int64_t total = block_prefix<kAttnThreads>(a, R, sm.pre, sm.sums);  // syncs the block
+  if (total == 0) return;
+  const int64_t W = workers_of(a, total);
+  volatile int* abort = &sm.abort;
+
+  if (warp == kAttnWarps) {
+    // lane w feeds warp w; lanes poll, none waits for another one's ring
+    const int64_t w = (int64_t)lane * gridDim.x + blockIdx.x;
+    Cursor c;
+    c.x = c.end = 0;
+    if (lane < kAttnWarps && w < W) {
+      c.x = total * w / W;
+      c.end = total * (w + 1) / W;
+    }
+    bool more = c.next(a, R, sm.pre);
+    uint32_t k = 0;  // records issued
+    int i = 0;
+    unsigned long long t0 = sm100::global_ns();
+    while (__any_sync(0xffffffffu, more)) {
+      if (more) {
+        const int st = k % S;
+        if (k < S || sm100::mbar_test(&sm.empty[lane][st], (k / S - 1) & 1)) {
+          const int blk = c.s.lo_blk + c.blk0 + i, h = c.unit / c.s.groups;
+          const uint8_t* rec =
+              blk * kBlock < c.s.len ? a.v.record(c.s.slot, blk, h) : nullptr;
+          sm.skip[lane][st] = rec == nullptr;
+          if (rec) {
+            sm100::mbar_arrive_expect_tx(&sm.full[lane][st], rec_bytes(D));
+            sm100::bulk_g2s(sm.ring[lane][st], rec, rec_bytes(D), &sm.full[lane][st]);
+          } else {
+            sm100::mbar_arrive(&sm.full[lane][st]);
+          }
+          ++k;
+          if (++i == c.n) {
+            i = 0;
+            more = c.next(a, R, sm.pre);
+          }
+          t0 = sm100::global_ns();
+        } else if (*abort || sm100::global_ns() - t0 > sm100::kWaitLimitNs) {
+          *abort = 1;
+          atomicOr(&g_status, 2);
+          more = false;
+        }
+      }
+      __syncwarp();
+    }
+    // the copies still in flight land before the block's memory is given up
+    for (int j = 0; j < S; ++j) {
+      const uint32_t q = k - 1 - j;
+      if (k == 0 || (uint32_t)j >= k) break;
+      t0 = sm100::global_ns();
+      while (!sm100::mbar_test(&sm.full[lane][q % S], (q / S) & 1) &&
+             sm100::global_ns() - t0 < sm100::kWaitLimitNs) {
+      }
+    }
+    return;
+  }
+
+  const int64_t w = (int64_t)warp * gridDim.x + blockIdx.x;
+  if (w >= W) return;
+  Cursor cur;
+  cur.x = total * w / W;
+  cur.end = total * (w + 1) / W;
+  const int g = lane >> 2, c = lane & 3;
+  uint32_t k = 0;
+  while (cur.next(a, R, sm.pre)) {
+    const Seq& s = cur.s;
+    const int n = cur.n, h = cur.unit / s.groups, row0 = cur.unit % s.groups * R;
     uint32_t qf[D / 16][NT][2];
     float qs[NT][2];
     load_q<D, NT, T>(a, s, h, row0, lane, qf, qs);
@@ -371,18 +486,22 @@ __global__ void __launch_bounds__(32 * kAttnWarps) attend_kernel(AttnArgs a) {
     const int see_lo = a.window > 0 ? last - a.window + 1 : 0;
     State<D, NT> st;
     st.clear();
-    for (int i = 0; i < n; ++i) {
-      const int blk = s.lo_blk + blk0 + i, t0 = blk * kBlock;
-      if (t0 >= s.len) continue;
-      const uint8_t* rec = a.v.record(s.slot, blk, h);
-      if (!rec) continue;
+    for (int i = 0; i < n; ++i, ++k) {
+      const int stage = k % S;
+      if (!sm100::mbar_wait(&sm.full[warp][stage], (k / S) & 1, abort)) return;
+      const uint8_t* rec = sm.ring[warp][stage];
       uint4 kc[D / 32], vc[D / 32];
 #pragma unroll
-      for (int k = 0; k < D / 32; ++k) {
-        kc[k] = *reinterpret_cast<const uint4*>(rec + 512 * k + 16 * lane);
-        vc[k] = *reinterpret_cast<const uint4*>(rec + 16 * D + 512 * k + 16 * lane);
+      for (int j = 0; j < D / 32; ++j) {
+        kc[j] = *reinterpret_cast<const uint4*>(rec + 512 * j + 16 * lane);
+        vc[j] = *reinterpret_cast<const uint4*>(rec + 16 * D + 512 * j + 16 * lane);
       }
       const float2 sc = *reinterpret_cast<const float2*>(rec + 32 * D);
+      const bool skip = sm.skip[warp][stage];
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&sm.empty[warp][stage]);
+      if (skip) continue;
+      const int t0 = (s.lo_blk + cur.blk0 + i) * kBlock;
       if (t0 >= see_lo && t0 + kBlock - 1 <= see_hi)
         block_step<D, KIND, NT, false>(st, kc, vc, sc.x, sc.y, qf, qs, t0, s.len, lo, hi, lane);
       else
@@ -398,13 +517,15 @@ __global__ void __launch_bounds__(32 * kAttnWarps) attend_kernel(AttnArgs a) {
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         st.l[t][r] = l;
       }
-    if (n == s.n_blk) {  // the whole unit: its rows are done
+    const bool whole = n == s.n_blk;  // the whole unit: its rows are done
+    float* p = a.part + (2 * w + (cur.blk0 == 0)) * part_floats(D, NT);
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int row = row0 + 8 * t + 2 * c + r;
-          if (row >= rows) continue;
+      for (int r = 0; r < 2; ++r) {
+        const int at_row = 8 * t + 2 * c + r, row = row0 + at_row;
+        if (row >= rows) continue;
+        if (whole) {
           const int64_t at = (s.r0 + row / a.group) * ((int64_t)a.v.heads * a.group) +
                              h * a.group + row % a.group;
           const float inv = st.l[t][r] == 0.f ? 0.f : __fdiv_rn(1.f, st.l[t][r]);
@@ -415,38 +536,40 @@ __global__ void __launch_bounds__(32 * kAttnWarps) attend_kernel(AttnArgs a) {
             out[16 * i + 8 + g] = from_float<T>(st.o[i][t][r + 2] * inv);
           }
           if (a.ml && g == 0) a.ml[at] = row_stats(st.m[t][r], st.m2[t][r], st.l[t][r]);
-        }
-    } else {
-      float* p = a.part + (2 * w + (blk0 == 0)) * part_floats(D, NT);
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int row = 8 * t + 2 * c + r;
+        } else {
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) {
-            p[row * D + 16 * i + g] = st.o[i][t][r];
-            p[row * D + 16 * i + 8 + g] = st.o[i][t][r + 2];
+            p[at_row * D + 16 * i + g] = st.o[i][t][r];
+            p[at_row * D + 16 * i + 8 + g] = st.o[i][t][r + 2];
           }
           if (g == 0)
-            *reinterpret_cast<float4*>(p + R * D + 4 * row) =
+            *reinterpret_cast<float4*>(p + R * D + 4 * at_row) =
                 make_float4(st.m2[t][r], st.l[t][r], st.m[t][r], 0.f);
         }
-    }
+      }
   }
 }
 
 // Joins the pieces of the units that several workers share, in the workers'
-// order: one CTA of D threads per (unit, row).
+// order: one CTA per (unit, row). The pieces' weights come first, 256 at a time,
+// then G = 256 / D groups of threads add every G-th piece.
+constexpr int kJoinThreads = 256;
+
 template <int D, int NT, typename T>
-__global__ void __launch_bounds__(D) attend_join_kernel(AttnArgs a) {
-  constexpr int R = 8 * NT;
-  extern __shared__ int64_t pre[];
-  const int64_t total = block_prefix<D>(a, R, pre, pre + a.v.B + 1);
+__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttnArgs a) {
+  constexpr int R = 8 * NT, G = kJoinThreads / D;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  int64_t* pre = reinterpret_cast<int64_t*>(smem_raw);
+  __shared__ int64_t sums[32];
+  __shared__ float weight[kJoinThreads], red[3][kJoinThreads / 32], acc[G][D];
+  // lengths and rows are not written by the kernel before: read ahead of the wait
+  const int64_t total = block_prefix<kJoinThreads>(a, R, pre, sums);
   const int64_t W = workers_of(a, total);
   const int64_t b = blockIdx.y;
   const Seq s = load_seq(a, b, R);
   const int unit = blockIdx.x / R, r = blockIdx.x % R;
+  wait_previous();
+  let_next_start();
   if (total == 0 || unit >= s.groups * a.v.heads) return;
   const int h = unit / s.groups, row = unit % s.groups * R + r;
   if (row >= s.n * a.group) return;
@@ -454,19 +577,52 @@ __global__ void __launch_bounds__(D) attend_join_kernel(AttnArgs a) {
   // worker w holds the blocks [total w / W, total (w + 1) / W)
   const int64_t w0 = ((x0 + 1) * W - 1) / total, w1 = (x1 * W - 1) / total;
   if (w0 == w1) return;
-  const int d = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, d = tid % D, grp = tid / D;
+  const int n = (int)(w1 - w0) + 1;
+  auto piece = [&](int i) {  // the first piece is its worker's last, the others their first
+    return a.part + (2 * (w0 + i) + (i == 0)) * part_floats(D, NT);
+  };
+  auto block_max = [&](float x, float* buf) {
+    x = warp_max(x);
+    if (lane == 0) buf[wid] = x;
+    __syncthreads();
+    x = buf[0];
+#pragma unroll
+    for (int i = 1; i < kJoinThreads / 32; ++i) x = fmaxf(x, buf[i]);
+    return x;
+  };
   float m = -INFINITY, m2 = -INFINITY, l = 0.f, o = 0.f;
-  for (int64_t w = w0; w <= w1; ++w) {
-    const bool from_start = w == w0;
-    const float* p = a.part + (2 * w + from_start) * part_floats(D, NT);
-    const float4 q = *reinterpret_cast<const float4*>(p + R * D + 4 * r);
-    const float now = fmaxf(m2, q.x), ref = now == -INFINITY ? 0.f : now;
-    const float f0 = exp2_approx(m2 - ref), f1 = exp2_approx(q.x - ref);
-    o = o * f0 + p[r * D + d] * f1;
-    l = l * f0 + q.y * f1;
+  for (int i = tid; i < n; i += kJoinThreads) {
+    const float4 q = *reinterpret_cast<const float4*>(piece(i) + R * D + 4 * r);
+    m2 = fmaxf(m2, q.x);
     m = fmaxf(m, q.z);
-    m2 = now;
   }
+  m2 = block_max(m2, red[0]);
+  m = block_max(m, red[1]);
+  const float ref = m2 == -INFINITY ? 0.f : m2;
+  for (int i0 = 0; i0 < n; i0 += kJoinThreads) {
+    __syncthreads();
+    if (i0 + tid < n) {
+      const float4 q = *reinterpret_cast<const float4*>(piece(i0 + tid) + R * D + 4 * r);
+      const float f = exp2_approx(q.x - ref);
+      weight[tid] = f;
+      l = fmaf(q.y, f, l);
+    }
+    __syncthreads();
+    const int k = min(kJoinThreads, n - i0);
+#pragma unroll 8
+    for (int i = grp; i < k; i += G) o = fmaf(piece(i0 + i)[r * D + d], weight[i], o);
+  }
+  l = warp_sum(l);
+  if (lane == 0) red[2][wid] = l;
+  acc[grp][d] = o;
+  __syncthreads();
+  if (grp) return;
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kJoinThreads / 32; ++i) l += red[2][i];
+#pragma unroll
+  for (int i = 1; i < G; ++i) o += acc[i][d];
   const int64_t at = (s.r0 + row / a.group) * ((int64_t)a.v.heads * a.group) + h * a.group +
                      row % a.group;
   ((T*)a.out)[at * D + d] = from_float<T>(l == 0.f ? 0.f : o * __fdiv_rn(1.f, l));
@@ -478,20 +634,40 @@ inline int row_tiles(int64_t max_new, int64_t group) { return max_new * group <=
 
 inline size_t attention_bytes(int64_t D, int64_t max_new, int64_t group) {
   const int NT = row_tiles(max_new, group);
-  return (size_t)2 * kSms * kAttnCtasPerSm * kAttnWarps * part_floats((int)D, NT) * sizeof(float);
+  return (size_t)2 * kSms * kAttnWarps * part_floats((int)D, NT) * sizeof(float);
+}
+
+template <typename... Params, typename... Args>
+static int launch_next(const char* what, void (*kernel)(Params...), dim3 grid, int threads,
+                       int smem, cudaStream_t st, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, args...);
+  return check_launch(what);
 }
 
 template <int D, int KIND, int NT, typename T>
 static int launch_attend(AttnArgs a, cudaStream_t st) {
-  const int smem = (int)((a.v.B + 1 + 32) * sizeof(int64_t));
   const int64_t groups = ((int64_t)a.max_new * a.group + 8 * NT - 1) / (8 * NT);
-  a.n_workers = kSms * kAttnCtasPerSm * kAttnWarps;
-  attend_kernel<D, KIND, NT, T><<<kSms * kAttnCtasPerSm, 32 * kAttnWarps, smem, st>>>(a);
-  int rc = check_launch("paged_attention");
+  a.n_workers = kSms * kAttnWarps;
+  const int smem = (int)(sizeof(AttnSmem<D>) + a.v.B * sizeof(int64_t));
+  // once per device would do; the call is cheap and keeps no state
+  cudaFuncSetAttribute(attend_kernel<D, KIND, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       (int)(sizeof(AttnSmem<D>) + kMaxSeqs * sizeof(int64_t)));
+  int rc = launch_next("paged_attention", attend_kernel<D, KIND, NT, T>, dim3(kSms), kAttnThreads,
+                       smem, st, a);
   if (rc) return rc;
   const dim3 grid((unsigned)(groups * a.v.heads * 8 * NT), (unsigned)a.v.B);
-  attend_join_kernel<D, NT, T><<<grid, D, smem, st>>>(a);
-  return check_launch("paged_attention (join)");
+  return launch_next("paged_attention (join)", attend_join_kernel<D, NT, T>, grid, kJoinThreads,
+                     (int)((a.v.B + 1) * sizeof(int64_t)), st, a);
 }
 
 }  // namespace paged

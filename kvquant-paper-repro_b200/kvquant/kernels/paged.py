@@ -29,12 +29,25 @@ import math
 
 import torch
 
-from .cuda_ops import _check, _ptr, _stream, get_cuda_ops
+from .cuda_ops import _check, _ptr, get_cuda_ops
 from .decode import DecodeWorkspace
 
 BLOCK_TOKENS = 16
 KINDS = {"int8": 0, "e4m3": 1}
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _launch(fn, lib, dev, *args) -> None:
+    """fn(*args, current stream of dev) with dev current. These calls take microseconds on
+    the GPU, so the device is switched only when it has to be."""
+    i = dev.index
+    if i == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc:
+        _check(rc, lib)
 
 
 def record_bytes(head_dim: int) -> int:
@@ -119,10 +132,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, table: to
     if k.shape != v.shape or k.dtype != v.dtype or _DTYPES.get(k.dtype, 2) == 2:
         raise RuntimeError("paged_append: k and v must have one shape and be fp16 or bf16")
     lib = get_cuda_ops().lib
-    with torch.cuda.device(dev):
-        _check(lib.kvq_paged_append(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+    _launch(lib.kvq_paged_append, lib, dev, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
                                     v.stride(0), v.stride(1), _DTYPES[k.dtype], *head, ip, B,
-                                    k.shape[0], _stream(pool)), lib)
+                                    k.shape[0])
 
 
 def paged_read(pool: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, kind: str,
@@ -133,13 +145,12 @@ def paged_read(pool: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, k
     head, ip, B = _cache_args("paged_read", pool, kind, table, lengths, slots, indptr, total)
     if dtype not in _DTYPES:
         raise RuntimeError(f"paged_read: dtype must be fp16, bf16 or fp32, got {dtype}")
-    k = torch.empty((int(total), head[3], head[4]), dtype=dtype, device=pool.device)
+    dev = pool.device
+    k = torch.empty((int(total), head[3], head[4]), dtype=dtype, device=dev)
     v = torch.empty_like(k)
     lib = get_cuda_ops().lib
-    with torch.cuda.device(pool.device):
-        _check(lib.kvq_paged_read(*head, _int32("paged_read", "starts", starts, pool.device, (B,)),
-                                  ip, B, int(total), k.data_ptr(), v.data_ptr(), _DTYPES[dtype],
-                                  _stream(pool)), lib)
+    _launch(lib.kvq_paged_read, lib, dev, *head, _int32("paged_read", "starts", starts, dev, (B,)),
+                                  ip, B, int(total), k.data_ptr(), v.data_ptr(), _DTYPES[dtype])
     return k, v
 
 
@@ -181,11 +192,10 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor,
     lib = get_cuda_ops().lib
     need = lib.kvq_paged_attention_workspace(dim, int(max_new), Hq // heads)
     ws = (workspace or DecodeWorkspace()).get(need, dev)
-    with torch.cuda.device(dev):
-        _check(lib.kvq_paged_attention(
+    _launch(lib.kvq_paged_attention, lib, dev, 
             q.data_ptr(), q.stride(0), q.stride(1), _DTYPES[q.dtype], Hq // heads, *head, ip, B, N,
             int(max_new), 1.0 / math.sqrt(dim) if scale is None else float(scale), int(window),
-            out.data_ptr(), _ptr(ml_out), ws.data_ptr(), ws.numel(), _stream(pool)), lib)
+            out.data_ptr(), _ptr(ml_out), ws.data_ptr(), ws.numel())
     return out
 
 
@@ -223,10 +233,8 @@ def paged_free(table, lengths, refs, slots, page_tokens: int, status) -> None:
     meta = _meta_args("paged_free", table, lengths, refs, page_tokens)
     dev = table.device
     lib = get_cuda_ops().lib
-    with torch.cuda.device(dev):
-        _check(lib.kvq_paged_free(*meta, _int32("paged_free", "slots", slots, dev), slots.numel(),
-                                  _int32("paged_free", "status", status, dev, (1,)),
-                                  _stream(table)), lib)
+    _launch(lib.kvq_paged_free, lib, dev, *meta, _int32("paged_free", "slots", slots, dev), slots.numel(),
+                                  _int32("paged_free", "status", status, dev, (1,)))
 
 
 def paged_fork(table, lengths, refs, src, dst, page_tokens: int, status) -> None:
@@ -236,11 +244,9 @@ def paged_fork(table, lengths, refs, src, dst, page_tokens: int, status) -> None
     meta = _meta_args("paged_fork", table, lengths, refs, page_tokens)
     dev = table.device
     lib = get_cuda_ops().lib
-    with torch.cuda.device(dev):
-        _check(lib.kvq_paged_fork(*meta, _int32("paged_fork", "src", src, dev),
+    _launch(lib.kvq_paged_fork, lib, dev, *meta, _int32("paged_fork", "src", src, dev),
                                   _int32("paged_fork", "dst", dst, dev, tuple(src.shape)),
-                                  src.numel(), _int32("paged_fork", "status", status, dev, (1,)),
-                                  _stream(table)), lib)
+                                  src.numel(), _int32("paged_fork", "status", status, dev, (1,)))
 
 
 def paged_extend(pool, table, lengths, refs, slots, n_new, status,
@@ -262,12 +268,11 @@ def paged_extend(pool, table, lengths, refs, slots, n_new, status,
     each = isinstance(n_new, torch.Tensor)
     lib = get_cuda_ops().lib
     ws = (workspace or DecodeWorkspace()).get(lib.kvq_paged_extend_workspace(refs.numel()), dev)
-    with torch.cuda.device(dev):
-        _check(lib.kvq_paged_extend(
+    _launch(lib.kvq_paged_extend, lib, dev, 
             ptr, layers, stride, page, *meta, _int32(what, "slots", slots, dev), slots.numel(),
             _int32(what, "n_new", n_new, dev, tuple(slots.shape)) if each else None,
             0 if each else int(n_new), _int32(what, "status", status, dev, (1,)), ws.data_ptr(),
-            ws.numel(), _stream(table)), lib)
+            ws.numel())
 
 
 def paged_compact(pool, table, refs, workspace: DecodeWorkspace | None = None,
@@ -284,12 +289,10 @@ def paged_compact(pool, table, refs, workspace: DecodeWorkspace | None = None,
         n_live = torch.empty(1, dtype=torch.int32, device=dev)
     lib = get_cuda_ops().lib
     ws = (workspace or DecodeWorkspace()).get(lib.kvq_paged_extend_workspace(refs.numel()), dev)
-    with torch.cuda.device(dev):
-        _check(lib.kvq_paged_compact(
+    _launch(lib.kvq_paged_compact, lib, dev, 
             ptr, layers, stride, page, _int32(what, "table", table, dev), table.shape[0],
             table.shape[1], _int32(what, "refs", refs, dev), refs.numel(),
-            _int32(what, "n_live", n_live, dev, (1,)), ws.data_ptr(), ws.numel(),
-            _stream(table)), lib)
+            _int32(what, "n_live", n_live, dev, (1,)), ws.data_ptr(), ws.numel())
     return n_live
 
 
@@ -305,8 +308,7 @@ def paged_copy(src_pool, dst_pool, src, dst, workspace: DecodeWorkspace | None =
     n = src.numel()
     lib = get_cuda_ops().lib
     ws = (workspace or DecodeWorkspace()).get(lib.kvq_paged_copy_workspace(n), dev)
-    with torch.cuda.device(dev):
-        _check(lib.kvq_paged_copy(
+    _launch(lib.kvq_paged_copy, lib, dev, 
             sp, src_pool.shape[-4], s_stride, dp, dst_pool.shape[-4], d_stride, layers, page,
             _int32(what, "src", src, dev), _int32(what, "dst", dst, dev, tuple(src.shape)), n,
-            ws.data_ptr(), ws.numel(), _stream(src_pool)), lib)
+            ws.data_ptr(), ws.numel())
