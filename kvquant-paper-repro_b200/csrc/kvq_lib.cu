@@ -10,3 +10,5 @@
 #include "kvq_codebook.cuh"
 #include "kvq_paged.cuh"
 #include "kvq_paged_attn.cuh"
+#include "kvq_paged_tile.cuh"
+#include "kvq_paged_api.cuh"

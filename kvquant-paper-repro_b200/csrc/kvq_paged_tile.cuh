@@ -1,0 +1,677 @@
+// Attention over the paged 8-bit KV cache for many query rows (prompt chunks,
+// drafted tokens): tcgen05 matrix products with TMEM accumulators. Part of the
+// kvq_lib.cu unity build; arithmetic as in kvq_paged_attn.cuh.
+//
+// A unit is 256 query rows (token, head of the group) of one KV head, in two
+// tiles of 128 rows that take turns on the tensor core: while one tile's softmax
+// runs, the other tile's products do. Keys and values come in tiles of 128
+// tokens:
+//   S_t = Q_t K^T          A = Q_t (shared), B = K (shared), both K-major
+//   O_t += P_t V           A = P_t (TMEM, over S_t's columns), B = V^T (shared)
+// Warps: 0-3 and 4-7 the softmax of tile 0 and 1 (a thread owns a row), 8-11 turn
+// records into fp16 tiles, 12 issues the products, 13 fetches records. The
+// record order makes each 4-byte value word a row segment of a core matrix, so
+// a warp writes whole 128-byte core matrices without bank conflicts.
+// One CTA per SM takes an equal share of all (unit, token tile) pairs; a unit
+// cut by a share's end is joined by tile_join_kernel. Bound by the tensor core
+// and the exponentials (128 x 128 per tile and half unit: 1024 cycles each).
+#pragma once
+#include "kvq_paged_attn.cuh"
+
+namespace kvq {
+namespace paged {
+
+constexpr int kTileRows = 128, kUnitRows = 256, kTileTok = 128;
+constexpr int kTileRecs = kTileTok / kBlock;  // records of a token tile
+constexpr int kRawStages = 12, kSlots = 3;
+constexpr int kTileThreads = 14 * 32;
+constexpr int kDequantWarp = 8, kMmaWarp = 12, kLoadWarp = 13;
+constexpr float kLazy = 8.f;  // the maximum may grow by 2^8 before O is rescaled
+
+template <int D>
+struct TileSmem {
+  alignas(128) uint8_t q[2][kTileRows * D * 2];
+  alignas(128) uint8_t slot[kSlots][kTileTok * D * 2];  // K and V tiles in turn
+  alignas(128) uint8_t raw[kRawStages][rec_bytes(D)];
+  uint64_t raw_full[kRawStages], raw_empty[kRawStages];
+  uint64_t slot_full[kSlots], slot_empty[kSlots];
+  uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain;
+  float4 scale[2][kTileRecs];  // (key scale, log2 value scale, 1 / value scale, -) of a tile
+  int64_t sums[32];
+  int skip[kRawStages];
+  uint32_t tmem;
+  int abort;
+  int32_t pre[1];  // B + 1
+};
+
+// Token tiles [t0, t0 + n) that row group r of a sequence sees (at least one).
+__device__ __forceinline__ void unit_tiles(const AttnArgs& a, const Seq& s, int r, int& t0,
+                                           int& n) {
+  const int p0 = s.len - s.n + (int)((int64_t)r * kUnitRows / a.group);
+  const int p1 = s.len - s.n +
+                 min(s.n - 1, (int)(((int64_t)r * kUnitRows + kUnitRows - 1) / a.group));
+  t0 = a.window > 0 ? max(0, p0 - a.window + 1) / kTileTok : 0;
+  n = max(1, max(p1, 0) / kTileTok - t0 + 1);
+}
+
+// As block_prefix, over token tiles.
+template <int THREADS>
+__device__ __forceinline__ int64_t tile_prefix(const AttnArgs& a, int32_t* pre, int64_t* sums) {
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  int64_t base = 0;
+  for (int64_t b0 = 0; b0 < a.v.B; b0 += THREADS) {
+    const int64_t b = b0 + threadIdx.x;
+    int64_t x = 0;
+    if (b < a.v.B) {
+      const Seq s = load_seq(a, b, kUnitRows);
+      for (int r = 0; r < s.groups; ++r) {
+        int t0, n;
+        unit_tiles(a, s, r, t0, n);
+        x += n;
+      }
+    }
+    int64_t incl = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) sums[wid] = incl;
+    __syncthreads();
+    int64_t before = base;
+    for (int i = 0; i < THREADS / 32; ++i) {
+      if (i < wid) before += sums[i];
+      base += sums[i];
+    }
+    if (b < a.v.B) pre[b] = (int32_t)(before + incl - x);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) pre[a.v.B] = (int32_t)base;
+  __syncthreads();
+  if (base > INT32_MAX) {  // more work than any call has: refused
+    if (threadIdx.x == 0) atomicOr(&g_status, kStatusBadIndex);
+    return 0;
+  }
+  return base * a.v.heads;
+}
+
+__device__ __forceinline__ int64_t tile_workers(int64_t total) {
+  return max((int64_t)1, min((int64_t)kSms, total));
+}
+
+struct TileCursor {
+  int64_t x, end;
+  Seq s;
+  int h, row0, t0, n_unit, first, n;  // piece: tiles [first, first + n) of the unit's n_unit
+  // Warp-collective.
+  __device__ bool next(const AttnArgs& a, const int32_t* pre, int lane) {
+    if (x >= end) return false;
+    int64_t lo = 0, hi = a.v.B;
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) >> 1;
+      if ((int64_t)pre[mid] * a.v.heads <= x) lo = mid;
+      else hi = mid;
+    }
+    s = load_seq(a, lo, kUnitRows);
+    const int64_t per = pre[lo + 1] - pre[lo];
+    const int64_t rem64 = x - (int64_t)pre[lo] * a.v.heads;
+    h = (int)(rem64 / per);
+    int rem = (int)(rem64 % per);
+    for (int r0 = 0;; r0 += 32) {
+      int mt0 = 0, mn = 0;
+      if (r0 + lane < s.groups) unit_tiles(a, s, r0 + lane, mt0, mn);
+      int incl = mn;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, incl > rem);
+      if (past || r0 + 32 >= s.groups) {
+        const int l = past ? __ffs(past) - 1 : 31;
+        t0 = __shfl_sync(0xffffffffu, mt0, l);
+        n_unit = __shfl_sync(0xffffffffu, mn, l);
+        first = rem - (__shfl_sync(0xffffffffu, incl, l) - n_unit);
+        row0 = (r0 + l) * kUnitRows;
+        break;
+      }
+      rem -= __shfl_sync(0xffffffffu, incl, 31);
+    }
+    n = (int)min((int64_t)(n_unit - first), end - x);
+    x += n;
+    return true;
+  }
+  __device__ int tiles(const AttnArgs& a) const {  // halves of the unit that have rows
+    return s.n * a.group - row0 > kTileRows ? 2 : 1;
+  }
+};
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
+        "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]),
+        "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
+      "%29, %30, %31, %32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+      "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
+      "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+      "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+      "r"(v[15])
+      : "memory");
+}
+
+// A query row to shared memory as fp16 (rows of the A operand, core matrices
+// [D / 8][row / 8]); returns the factor of its scores. Negative softmax scales
+// turn the row's sign, so the factor is >= 0 and maxima keep their meaning.
+template <int D, typename T>
+__device__ __forceinline__ float stage_q(const AttnArgs& a, const T* p, bool valid, uint8_t* q,
+                                         int row) {
+  uint4 w[D / 8];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i)
+    w[i] = valid ? *reinterpret_cast<const uint4*>(p + 8 * i) : make_uint4(0, 0, 0, 0);
+  float f = 1.f, inv = 1.f;
+  if constexpr (!std::is_same<T, __half>::value) {
+    float mx = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 y = to_float2<T>(x[e]);
+        mx = fmaxf(mx, fmaxf(fabsf(y.x), fabsf(y.y)));
+      }
+    }
+    const int e = max(-100, (int)((__float_as_uint(mx) >> 23) & 255) - 127);
+    if (mx > 0.f && mx < INFINITY) {
+      f = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+      inv = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+    }
+  }
+  const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) {
+    uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (!std::is_same<T, __half>::value) {
+        const float2 y = to_float2<T>(x[e]);
+        x[e] = half2_bits(y.x * f, y.y * f);
+      }
+      x[e] ^= sign;
+    }
+    *reinterpret_cast<uint4*>(q + i * (kTileRows * 16) + (row >> 3) * 128 + (row & 7) * 16) =
+        make_uint4(x[0], x[1], x[2], x[3]);
+  }
+  return fabsf(a.scale_log2) * inv;
+}
+
+template <int D, int KIND, typename T>
+__global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a) {
+  using namespace sm100;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  TileSmem<D>& sm = *reinterpret_cast<TileSmem<D>*>(smem_raw);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  volatile int* abort = &sm.abort;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kRawStages; ++i) {
+      mbar_init(&sm.raw_full[i], 1);
+      mbar_init(&sm.raw_empty[i], 1);
+    }
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&sm.slot_full[i], 4);
+      mbar_init(&sm.slot_empty[i], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&sm.q_full[t], kTileRows);
+      mbar_init(&sm.s_full[t], 1);
+      mbar_init(&sm.p_full[t], kTileRows);
+      mbar_init(&sm.o_full[t], 1);
+    }
+    mbar_init(&sm.drain, 1);
+    *abort = 0;
+    fence_mbar_init();
+  }
+  wait_previous();
+  let_next_start();
+  const int64_t total = tile_prefix<kTileThreads>(a, sm.pre, sm.sums);  // syncs the block
+  const int64_t W = tile_workers(total);
+  if (total == 0 || blockIdx.x >= W) return;
+  if (warp == kMmaWarp) tmem_alloc(&sm.tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+  const uint32_t tmem_s[2] = {tmem, tmem + kTileTok};
+  const uint32_t tmem_o[2] = {tmem + 2 * kTileTok, tmem + 2 * kTileTok + D};
+  TileCursor c;
+  c.x = total * blockIdx.x / W;
+  c.end = total * (blockIdx.x + 1) / W;
+  uint32_t gi = 0;  // token tiles before the current one
+
+  auto load_role = [&]() {
+    uint32_t issued = 0;
+    const int j = lane;
+    bool ok = true;
+    while (ok && c.next(a, sm.pre, lane)) {
+      for (int i = 0; ok && i < c.n; ++i, ++gi) {
+        const uint32_t k = gi * kTileRecs + j, st = k % kRawStages, use = k / kRawStages;
+        if (j < kTileRecs) {
+          const unsigned long long t0 = global_ns();
+          while (use > 0 && !mbar_test(&sm.raw_empty[st], (use - 1) & 1)) {
+            if (*abort || global_ns() - t0 > kWaitLimitNs) {
+              *abort = 1;
+              atomicOr(&g_status, 2);
+              ok = false;
+              break;
+            }
+          }
+          if (ok) {
+            const int blk = (c.t0 + c.first + i) * kTileRecs + j;
+            const uint8_t* rec =
+                blk * kBlock < c.s.len ? a.v.record(c.s.slot, blk, c.h) : nullptr;
+            sm.skip[st] = rec == nullptr;
+            if (rec) {
+              mbar_arrive_expect_tx(&sm.raw_full[st], rec_bytes(D));
+              bulk_g2s(sm.raw[st], rec, rec_bytes(D), &sm.raw_full[st]);
+            } else {
+              mbar_arrive(&sm.raw_full[st]);
+            }
+            issued = k + 1;
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+      }
+    }
+    // the copies in flight land before the block ends: each stage's last record,
+    // i.e. those that no later one (12 on) has followed into the stage
+    const uint32_t last = __reduce_max_sync(0xffffffffu, issued);
+    for (uint32_t b = 0; b < 2 && j < kTileRecs && issued > b * kTileRecs; ++b) {
+      const uint32_t k = issued - 1 - b * kTileRecs;
+      if (k + kRawStages < last) break;
+      const unsigned long long t0 = global_ns();
+      while (!mbar_test(&sm.raw_full[k % kRawStages], (k / kRawStages) & 1) &&
+             global_ns() - t0 < kWaitLimitNs) {
+      }
+    }
+    __syncwarp();
+  };
+
+  auto dequant_role = [&]() {
+    const int dw = warp - kDequantWarp, g = lane >> 2, cc = lane & 3;
+    while (c.next(a, sm.pre, lane)) {
+      for (int i = 0; i < c.n; ++i, ++gi) {
+        const int tok0 = (c.t0 + c.first + i) * kTileTok;
+        bool skip[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int j = dw + 4 * u;
+          const uint32_t k = gi * kTileRecs + j, st = k % kRawStages;
+          if (!mbar_wait(&sm.raw_full[st], (k / kRawStages) & 1, abort)) return;
+          skip[u] = sm.skip[st];
+        }
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const uint32_t q = 2 * gi + kv, slot = q % kSlots, use = q / kSlots;
+          if (use > 0 && !mbar_wait(&sm.slot_empty[slot], (use - 1) & 1, abort)) return;
+          uint8_t* out = sm.slot[slot];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int j = dw + 4 * u;
+            const uint8_t* rec = sm.raw[(gi * kTileRecs + j) % kRawStages];
+            if (kv == 0 && lane == 0) {
+              const float2 sc = *reinterpret_cast<const float2*>(rec + 32 * D);
+              sm.scale[gi & 1][j] = skip[u] ? make_float4(0.f, -INFINITY, 0.f, 0.f)
+                                            : make_float4(sc.x, __log2f(sc.y),
+                                                          __fdividef(1.f, sc.y), 0.f);
+            }
+            uint32_t vmask = 0xffffffffu;
+            if (KIND == kE4m3 && kv == 1 && tok0 + kBlock * j + kBlock > c.s.len) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (tok0 + kBlock * j + 2 * cc + (e & 1) + 8 * (e >> 1) >= c.s.len)
+                  vmask &= ~(0xffu << (8 * e));
+            }
+#pragma unroll
+            for (int m = 0; m < D / 32; ++m) {
+              const uint4 x =
+                  *reinterpret_cast<const uint4*>(rec + kv * 16 * D + 512 * m + 16 * lane);
+              const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                uint32_t lo, hi;
+                code_halves<KIND>(kv ? w[e] & vmask : w[e], lo, hi);
+                if (skip[u]) lo = hi = 0;
+                if (kv == 0) {
+                  // token 8 (2 j + (e & 1)) + g, channels 32 m + 16 (e >> 1) + 4 cc ..
+                  const int tg = 2 * j + (e & 1), cg = 4 * m + 2 * (e >> 1) + (cc >> 1);
+                  *reinterpret_cast<uint2*>(out + (tg * (D / 8) + cg) * 128 + g * 16 +
+                                            (cc & 1) * 8) = make_uint2(lo, hi);
+                } else {
+                  // channel 32 m + 8 e + g, tokens 16 j + 2 cc, + 1 and those + 8
+                  const int cg = 4 * m + e;
+                  *reinterpret_cast<uint32_t*>(out + (2 * j * (D / 8) + cg) * 128 + g * 16 +
+                                               cc * 4) = lo;
+                  *reinterpret_cast<uint32_t*>(out + ((2 * j + 1) * (D / 8) + cg) * 128 + g * 16 +
+                                               cc * 4) = hi;
+                }
+              }
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&sm.slot_full[slot]);
+            if (kv == 1) {
+              mbar_arrive(&sm.raw_empty[(gi * kTileRecs + dw) % kRawStages]);
+              mbar_arrive(&sm.raw_empty[(gi * kTileRecs + dw + 4) % kRawStages]);
+            }
+          }
+        }
+      }
+    }
+  };
+
+  auto mma_role = [&]() {
+    constexpr uint32_t id_s = idesc_f16_f32(kTileRows, kTileTok);
+    constexpr uint32_t id_o = idesc_f16_f32(kTileRows, D);
+    uint32_t n_q[2] = {0, 0}, n_p[2] = {0, 0};
+    auto scores = [&](int t, uint32_t slot) {
+      if (lane == 0) {
+        const uint64_t qd = smem_desc(smem_addr(sm.q[t]), kTileRows * 16, 128);
+        const uint64_t kd = smem_desc(smem_addr(sm.slot[slot]), 128, D * 16);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          mma_f16_ss(tmem_s[t], qd + k * (2 * kTileRows * 16 / 16), kd + k * (256 / 16), id_s,
+                     k > 0);
+        mma_commit(&sm.s_full[t]);
+      }
+      __syncwarp();
+    };
+    while (c.next(a, sm.pre, lane)) {
+      const int nt = c.tiles(a);
+      for (int i = 0; i < c.n; ++i, ++gi) {
+        const uint32_t ks = (2 * gi) % kSlots, ku = (2 * gi) / kSlots;
+        const uint32_t vs = (2 * gi + 1) % kSlots, vu = (2 * gi + 1) / kSlots;
+        const uint32_t ns = (2 * gi + 2) % kSlots, nu = (2 * gi + 2) / kSlots;
+        if (i == 0) {
+          if (!mbar_wait(&sm.slot_full[ks], ku & 1, abort)) return;
+          for (int t = 0; t < nt; ++t) {
+            if (!mbar_wait(&sm.q_full[t], n_q[t]++ & 1, abort)) return;
+            tc_fence_after();
+            scores(t, ks);
+          }
+          if (lane == 0) mma_commit(&sm.slot_empty[ks]);
+          __syncwarp();
+        }
+        if (!mbar_wait(&sm.slot_full[vs], vu & 1, abort)) return;
+        for (int t = 0; t < nt; ++t) {
+          if (!mbar_wait(&sm.p_full[t], n_p[t]++ & 1, abort)) return;
+          tc_fence_after();
+          if (lane == 0) {
+            const uint64_t vd = smem_desc(smem_addr(sm.slot[vs]), D * 16, 128);
+#pragma unroll
+            for (int k = 0; k < kTileTok / 16; ++k)
+              mma_f16_ts(tmem_o[t], tmem_s[t] + 8 * k, vd + k * (2 * D * 16 / 16), id_o,
+                         i > 0 || k > 0);
+            if (t == nt - 1) mma_commit(&sm.slot_empty[vs]);
+            if (i + 1 == c.n) mma_commit(&sm.o_full[t]);
+          }
+          __syncwarp();
+          if (i + 1 < c.n) {
+            if (t == 0 && !mbar_wait(&sm.slot_full[ns], nu & 1, abort)) return;
+            scores(t, ns);
+            if (t == nt - 1 && lane == 0) mma_commit(&sm.slot_empty[ns]);
+            __syncwarp();
+          }
+        }
+      }
+    }
+  };
+
+  auto softmax_role = [&]() {
+    const int t = warp >> 2, row = threadIdx.x & 127;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane 32 (warp % 4)
+    const uint32_t ts = tmem_s[t] + lanes, to = tmem_o[t] + lanes;
+    uint32_t n_s = 0, n_o = 0;
+    while (c.next(a, sm.pre, lane)) {
+      if (t >= c.tiles(a)) {
+        gi += c.n;
+        continue;
+      }
+      const Seq& s = c.s;
+      const int r = c.row0 + kTileRows * t + row, rows = s.n * a.group;
+      const bool valid = r < rows;
+      const int tok = valid ? r / a.group : 0;
+      const int head = c.h * a.group + r % a.group;
+      const float qs = stage_q<D, T>(
+          a, (const T*)a.q + (s.r0 + tok) * a.q_tok + (int64_t)head * a.q_head, valid, sm.q[t],
+          row);
+      fence_proxy_async_smem();
+      mbar_arrive(&sm.q_full[t]);
+      // a row sees the tokens lo .. hi; rows past the end mask nothing and are not stored
+      const int pos = s.len - s.n + tok;
+      const int hi = valid ? pos : INT_MAX;
+      const int lo = valid && a.window > 0 ? max(0, pos - a.window + 1) : 0;
+      const bool idle = !__any_sync(0xffffffffu, valid);
+      float m = -INFINITY, ref = -INFINITY, l = 0.f;
+      for (int i = 0; i < c.n; ++i, ++gi) {
+        if (!mbar_wait(&sm.s_full[t], n_s++ & 1, abort)) return;
+        tc_fence_after();
+        if (!idle) {
+          const int j0 = (c.t0 + c.first + i) * kTileTok;
+          const bool masked = __any_sync(0xffffffffu, j0 < lo || j0 + kTileTok - 1 > hi);
+          const float4* sc = sm.scale[gi & 1];
+          float top = -INFINITY;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t x[32];
+            tmem_ld32(ts + 32 * q, x);
+            tmem_wait_ld();
+            if (masked) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const int j = j0 + 32 * q + e;
+                if (j < lo || j > hi) x[e] = 0xff800000u;
+              }
+            }
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              float bm = __uint_as_float(x[16 * b]);
+#pragma unroll
+              for (int e = 1; e < 16; ++e) bm = fmaxf(bm, __uint_as_float(x[16 * b + e]));
+              const float4 f = sc[2 * q + b];
+              const float tm = f.y == -INFINITY || bm == -INFINITY ? -INFINITY : bm * (f.x * qs);
+              m = fmaxf(m, tm);
+              top = fmaxf(top, tm + f.y);
+            }
+          }
+          const bool grow = top > ref + kLazy || (ref == -INFINITY && top > ref);
+          if (__any_sync(0xffffffffu, grow)) {
+            const float now = fmaxf(ref, top);
+            const float alpha = now == -INFINITY ? 1.f : exp2_approx(ref - now);
+            ref = now;
+            l *= alpha;
+            if (i > 0) {
+#pragma unroll
+              for (int q = 0; q < D / 32; ++q) {
+                uint32_t x[32];
+                tmem_ld32(to + 32 * q, x);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  x[e] = __float_as_uint(__uint_as_float(x[e]) * alpha);
+                tmem_st32(to + 32 * q, x);
+              }
+            }
+          }
+          const float base = ref == -INFINITY ? 0.f : ref;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t x[32], p[16];
+            tmem_ld32(ts + 32 * q, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              const float4 f = sc[2 * q + b];
+              const float fk = f.x * qs, fv = f.y - base;
+              float sum = 0.f;
+#pragma unroll
+              for (int e = 0; e < 16; e += 2) {
+                float y[2];
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                  y[z] = fmaf(__uint_as_float(x[16 * b + e + z]), fk, fv);
+                  if (masked) {
+                    const int j = j0 + 32 * q + 16 * b + e + z;
+                    if (j < lo || j > hi) y[z] = -INFINITY;
+                  }
+                  y[z] = exp2_approx(y[z]);
+                  sum += y[z];
+                }
+                p[8 * b + e / 2] = half2_bits(y[0], y[1]);
+              }
+              l = fmaf(sum, f.z, l);
+            }
+            tmem_st16(ts + 16 * q, p);
+          }
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        mbar_arrive(&sm.p_full[t]);
+      }
+      if (!mbar_wait(&sm.o_full[t], n_o++ & 1, abort)) return;
+      tc_fence_after();
+      if (idle) continue;
+      const bool whole = c.n == c.n_unit;
+      const float inv = !whole ? 1.f : l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+      const int64_t at = (s.r0 + tok) * ((int64_t)a.v.heads * a.group) + head;
+      float* part = a.part + (2 * (int64_t)blockIdx.x + (c.first == 0)) * (kUnitRows * (D + 4));
+      const int ur = kTileRows * t + row;
+#pragma unroll
+      for (int q = 0; q < D / 32; ++q) {
+        uint32_t x[32];
+        tmem_ld32(to + 32 * q, x);
+        tmem_wait_ld();
+        if (valid && whole) {
+          T* out = (T*)a.out + at * D + 32 * q;
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            float y[8];
+#pragma unroll
+            for (int z = 0; z < 8; ++z) y[z] = l == 0.f ? 0.f : __uint_as_float(x[e + z]) * inv;
+            store8<T>(out + e, y);
+          }
+        } else if (valid) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<uint4*>(part + ur * D + 32 * q + e) =
+                make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+        }
+      }
+      if (valid && whole) {
+        if (a.ml) a.ml[at] = row_stats(m, ref, l);
+      } else if (valid) {
+        *reinterpret_cast<float4*>(part + kUnitRows * D + 4 * ur) = make_float4(ref, l, m, 0.f);
+      }
+    }
+  };
+
+  if (warp == kLoadWarp) load_role();
+  else if (warp == kMmaWarp) mma_role();
+  else if (warp >= kDequantWarp) dequant_role();
+  else softmax_role();
+
+  __syncwarp();
+  if (warp == kMmaWarp) {  // products still in flight (after an abort) end first
+    if (lane == 0) mma_commit(&sm.drain);
+    __syncwarp();
+    mbar_wait(&sm.drain, 0, abort, false);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+}
+
+// Joins a unit that the shares' ends cut: the CTA column of the unit's first
+// inner cut adds its pieces in order, 32 rows per CTA.
+constexpr int kTileJoinRows = 32;
+
+template <int D, typename T>
+__global__ void __launch_bounds__(kJoinThreads) tile_join_kernel(AttnArgs a) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  int32_t* pre = reinterpret_cast<int32_t*>(smem_raw);
+  __shared__ int64_t sums[32];
+  const int64_t total = tile_prefix<kJoinThreads>(a, pre, sums);
+  // every CTA waits, or a later launch could pass the attention kernel
+  wait_previous();
+  let_next_start();
+  const int64_t W = tile_workers(total), cut = blockIdx.x + 1;
+  if (total == 0 || cut >= W) return;
+  TileCursor c;
+  c.x = total * cut / W;
+  c.end = total;
+  const int64_t x = c.x;
+  c.next(a, pre, threadIdx.x & 31);
+  const int64_t start = x - c.first, end = start + c.n_unit;
+  if (c.first == 0 || total * (cut - 1) / W > start) return;
+  constexpr int G = kJoinThreads / D, F = kUnitRows * (D + 4);
+  const int d = threadIdx.x % D;
+  for (int i = threadIdx.x / D; i < kTileJoinRows; i += G) {
+    const int ur = blockIdx.y * kTileJoinRows + i, r = c.row0 + ur;
+    if (r >= c.s.n * a.group) return;
+    float m = -INFINITY, ref = -INFINITY, l = 0.f, o = 0.f;
+    for (int64_t w = cut - 1; w < W && total * w / W < end; ++w) {
+      const float* p = a.part + (2 * w + (w == cut - 1)) * F;
+      const float4 q = *reinterpret_cast<const float4*>(p + kUnitRows * D + 4 * ur);
+      const float now = fmaxf(ref, q.x), base = now == -INFINITY ? 0.f : now;
+      const float f0 = exp2_approx(ref - base), f1 = exp2_approx(q.x - base);
+      o = o * f0 + p[ur * D + d] * f1;
+      l = l * f0 + q.y * f1;
+      m = fmaxf(m, q.z);
+      ref = now;
+    }
+    const int64_t at = (c.s.r0 + r / a.group) * ((int64_t)a.v.heads * a.group) +
+                       c.h * a.group + r % a.group;
+    ((T*)a.out)[at * D + d] = from_float<T>(l == 0.f ? 0.f : o * __fdiv_rn(1.f, l));
+    if (a.ml && d == 0) a.ml[at] = row_stats(m, ref, l);
+  }
+}
+
+template <int D, int KIND, typename T>
+static int launch_attend_tile(AttnArgs a, cudaStream_t st) {
+  const int smem = (int)(sizeof(TileSmem<D>) + a.v.B * sizeof(int32_t));
+  cudaFuncSetAttribute(attend_tile_kernel<D, KIND, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       (int)(sizeof(TileSmem<D>) + kMaxSeqs * sizeof(int32_t)));
+  int rc = launch_next("paged_attention (tiles)", attend_tile_kernel<D, KIND, T>, dim3(kSms),
+                       kTileThreads, smem, st, a);
+  if (rc) return rc;
+  return launch_next("paged_attention (tile join)", tile_join_kernel<D, T>,
+                     dim3(kSms - 1, kUnitRows / kTileJoinRows), kJoinThreads,
+                     (int)((a.v.B + 1) * sizeof(int32_t)), st, a);
+}
+
+}  // namespace paged
+}  // namespace kvq

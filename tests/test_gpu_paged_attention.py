@@ -235,3 +235,14 @@ def test_bad_indices_are_reported_and_skipped(cuda):
         with pytest.raises(RuntimeError, match="out of range"):
             ops.check_status(cuda)
         assert torch.equal(got[1], good[1]), what
+
+
+@pytest.mark.parametrize("kind,D,G,lens,new,window", [
+    ("int8", 128, 4, [2600] * 6, [70] * 6, 0),        # many token tiles and units per SM
+    ("e4m3", 64, 4, [1800, 2900, 5, 700] * 4, [5] * 16, 1000),
+    ("int8", 64, 8, [900] * 8, [17, 40, 33, 64, 3, 0, 100, 900], 0),
+])
+def test_many_tiles_per_sm(cuda, kind, D, G, lens, new, window):
+    """More work than one token tile per SM: rings and slots are used many times over."""
+    c = Cache(lens, H=3, D=D, page=32, kind=kind, dtype="bf16", seed=D + G)
+    compare(cuda, c, new, G, window=window)
