@@ -227,6 +227,121 @@ __device__ __forceinline__ float stage_q(const AttnArgs& a, const T* p, bool val
   return fabsf(a.scale_log2) * inv;
 }
 
+// Two fp32 operations in one instruction (each rounded as the scalar one).
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Softmax state of a thread's row: the maximum of the scores, the reference of
+// the weights and the sum relative to it (log2 units).
+struct RowState {
+  float m, ref, l;
+};
+
+// One tile of a row: scores from TMEM, weights back over the first half of their
+// columns. MASK: some row of the warp does not see all 128 tokens; the row sees
+// the columns c with (unsigned)(c + first) <= span.
+template <int D, bool MASK>
+__device__ __forceinline__ void softmax_tile(RowState& st, uint32_t ts, uint32_t to, bool has_o,
+                                             const float4* sc, float qs, int first,
+                                             uint32_t span) {
+  using namespace sm100;
+  float top = -INFINITY;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t x[32];
+    tmem_ld32(ts + 32 * q, x);
+    tmem_wait_ld();
+    if (MASK) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if ((uint32_t)(first + 32 * q + e) > span) x[e] = 0xff800000u;
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const uint32_t* y = x + 16 * b;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(y[e]);
+#pragma unroll
+      for (int e = 4; e < 16; e += 4)
+#pragma unroll
+        for (int z = 0; z < 4; ++z) v[z] = fmaxf(v[z], __uint_as_float(y[e + z]));
+      const float bm = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+      const float4 f = sc[2 * q + b];
+      const float tm = f.y == -INFINITY || bm == -INFINITY ? -INFINITY : bm * (f.x * qs);
+      st.m = fmaxf(st.m, tm);
+      top = fmaxf(top, tm + f.y);
+    }
+  }
+  if (__any_sync(0xffffffffu, top > st.ref + kLazy)) {
+    const float now = fmaxf(st.ref, top);
+    const float alpha = now == -INFINITY ? 1.f : exp2_approx(st.ref - now);
+    st.ref = now;
+    st.l *= alpha;
+    if (has_o) {
+#pragma unroll 1
+      for (int q = 0; q < D / 32; ++q) {
+        uint32_t x[32];
+        tmem_ld32(to + 32 * q, x);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * alpha);
+        tmem_st32(to + 32 * q, x);
+      }
+    }
+  }
+  const float base = st.ref == -INFINITY ? 0.f : st.ref;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t x[32], p[16];
+    tmem_ld32(ts + 32 * q, x);
+    tmem_wait_ld();
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const float4 f = sc[2 * q + b];
+      const float fk = f.x * qs, fv = f.y - base;
+      const uint64_t fk2 = pack2(fk, fk), fv2 = pack2(fv, fv);
+      uint64_t sum[2] = {0, 0};
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        float y0, y1;
+        unpack2(fma2(pack2(__uint_as_float(x[16 * b + e]), __uint_as_float(x[16 * b + e + 1])),
+                     fk2, fv2),
+                y0, y1);
+        if (MASK) {
+          if ((uint32_t)(first + 32 * q + 16 * b + e) > span) y0 = -INFINITY;
+          if ((uint32_t)(first + 32 * q + 16 * b + e + 1) > span) y1 = -INFINITY;
+        }
+        y0 = exp2_approx(y0);
+        y1 = exp2_approx(y1);
+        sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(y0, y1));
+        p[8 * b + e / 2] = half2_bits(y0, y1);
+      }
+      float s0, s1;
+      unpack2(add2(sum[0], sum[1]), s0, s1);
+      st.l = fmaf(s0 + s1, f.z, st.l);
+    }
+    tmem_st16(ts + 16 * q, p);
+  }
+  tmem_wait_st();
+}
+
 template <int D, int KIND, typename T>
 __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a) {
   using namespace sm100;
@@ -470,93 +585,28 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
           row);
       fence_proxy_async_smem();
       mbar_arrive(&sm.q_full[t]);
-      // a row sees the tokens lo .. hi; rows past the end mask nothing and are not stored
+      // a row sees the tokens lo .. lo + span; rows past the end mask nothing and are
+      // not stored; a row before the first token sees none
       const int pos = s.len - s.n + tok;
-      const int hi = valid ? pos : INT_MAX;
-      const int lo = valid && a.window > 0 ? max(0, pos - a.window + 1) : 0;
+      int lo = 0;
+      uint32_t span = INT_MAX;
+      if (valid) {
+        lo = pos < 0 ? INT_MAX : a.window > 0 ? max(0, pos - a.window + 1) : 0;
+        span = pos < 0 ? 0 : pos - lo;
+      }
       const bool idle = !__any_sync(0xffffffffu, valid);
-      float m = -INFINITY, ref = -INFINITY, l = 0.f;
+      RowState st = {-INFINITY, -INFINITY, 0.f};
       for (int i = 0; i < c.n; ++i, ++gi) {
         if (!mbar_wait(&sm.s_full[t], n_s++ & 1, abort)) return;
         tc_fence_after();
         if (!idle) {
-          const int j0 = (c.t0 + c.first + i) * kTileTok;
-          const bool masked = __any_sync(0xffffffffu, j0 < lo || j0 + kTileTok - 1 > hi);
-          const float4* sc = sm.scale[gi & 1];
-          float top = -INFINITY;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t x[32];
-            tmem_ld32(ts + 32 * q, x);
-            tmem_wait_ld();
-            if (masked) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const int j = j0 + 32 * q + e;
-                if (j < lo || j > hi) x[e] = 0xff800000u;
-              }
-            }
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              float bm = __uint_as_float(x[16 * b]);
-#pragma unroll
-              for (int e = 1; e < 16; ++e) bm = fmaxf(bm, __uint_as_float(x[16 * b + e]));
-              const float4 f = sc[2 * q + b];
-              const float tm = f.y == -INFINITY || bm == -INFINITY ? -INFINITY : bm * (f.x * qs);
-              m = fmaxf(m, tm);
-              top = fmaxf(top, tm + f.y);
-            }
-          }
-          const bool grow = top > ref + kLazy || (ref == -INFINITY && top > ref);
-          if (__any_sync(0xffffffffu, grow)) {
-            const float now = fmaxf(ref, top);
-            const float alpha = now == -INFINITY ? 1.f : exp2_approx(ref - now);
-            ref = now;
-            l *= alpha;
-            if (i > 0) {
-#pragma unroll
-              for (int q = 0; q < D / 32; ++q) {
-                uint32_t x[32];
-                tmem_ld32(to + 32 * q, x);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  x[e] = __float_as_uint(__uint_as_float(x[e]) * alpha);
-                tmem_st32(to + 32 * q, x);
-              }
-            }
-          }
-          const float base = ref == -INFINITY ? 0.f : ref;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t x[32], p[16];
-            tmem_ld32(ts + 32 * q, x);
-            tmem_wait_ld();
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              const float4 f = sc[2 * q + b];
-              const float fk = f.x * qs, fv = f.y - base;
-              float sum = 0.f;
-#pragma unroll
-              for (int e = 0; e < 16; e += 2) {
-                float y[2];
-#pragma unroll
-                for (int z = 0; z < 2; ++z) {
-                  y[z] = fmaf(__uint_as_float(x[16 * b + e + z]), fk, fv);
-                  if (masked) {
-                    const int j = j0 + 32 * q + 16 * b + e + z;
-                    if (j < lo || j > hi) y[z] = -INFINITY;
-                  }
-                  y[z] = exp2_approx(y[z]);
-                  sum += y[z];
-                }
-                p[8 * b + e / 2] = half2_bits(y[0], y[1]);
-              }
-              l = fmaf(sum, f.z, l);
-            }
-            tmem_st16(ts + 16 * q, p);
-          }
-          tmem_wait_st();
+          const int first = (c.t0 + c.first + i) * kTileTok - lo;
+          const bool masked = __any_sync(
+              0xffffffffu, first < 0 || (uint32_t)(first + kTileTok - 1) > span);
+          if (masked)
+            softmax_tile<D, true>(st, ts, to, i > 0, sm.scale[gi & 1], qs, first, span);
+          else
+            softmax_tile<D, false>(st, ts, to, i > 0, sm.scale[gi & 1], qs, first, span);
         }
         tc_fence_before();
         mbar_arrive(&sm.p_full[t]);
@@ -564,6 +614,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
       if (!mbar_wait(&sm.o_full[t], n_o++ & 1, abort)) return;
       tc_fence_after();
       if (idle) continue;
+      const float l = st.l;
       const bool whole = c.n == c.n_unit;
       const float inv = !whole ? 1.f : l == 0.f ? 0.f : __fdiv_rn(1.f, l);
       const int64_t at = (s.r0 + tok) * ((int64_t)a.v.heads * a.group) + head;
@@ -591,9 +642,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
         }
       }
       if (valid && whole) {
-        if (a.ml) a.ml[at] = row_stats(m, ref, l);
+        if (a.ml) a.ml[at] = row_stats(st.m, st.ref, l);
       } else if (valid) {
-        *reinterpret_cast<float4*>(part + kUnitRows * D + 4 * ur) = make_float4(ref, l, m, 0.f);
+        *reinterpret_cast<float4*>(part + kUnitRows * D + 4 * ur) = make_float4(st.ref, l, st.m, 0.f);
       }
     }
   };
