@@ -24,7 +24,11 @@ namespace paged {
 constexpr int kTileRows = 128, kUnitRows = 256, kTileTok = 128;
 constexpr int kTileRecs = kTileTok / kBlock;  // records of a token tile
 constexpr int kRawStages = 12, kSlots = 3;
-constexpr int kTileThreads = 14 * 32;
+constexpr int kTileThreads = 16 * 32;  // warps 14 and 15 only complete their warpgroup
+// Registers per thread of the warpgroups (softmax twice, dequantising, products and
+// copies): together the 4 x 128 of the launch. The softmax keeps a row's 128 scores.
+constexpr int kRegsSoftmax = 184, kRegsDequant = 96, kRegsIssue = 48;
+static_assert(2 * kRegsSoftmax + kRegsDequant + kRegsIssue <= 4 * 128, "register shares");
 constexpr int kDequantWarp = 8, kMmaWarp = 12, kLoadWarp = 13;
 constexpr float kLazy = 8.f;  // the maximum may grow by 2^8 before O is rescaled
 
@@ -159,18 +163,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
-      "%29, %30, %31, %32};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
-      "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
-      "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
-      "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
@@ -262,19 +254,20 @@ __device__ __forceinline__ void softmax_tile(RowState& st, uint32_t ts, uint32_t
                                              uint32_t span) {
   using namespace sm100;
   float top = -INFINITY;
+  uint32_t x[4][32];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) tmem_ld32(ts + 32 * q, x[q]);
+  tmem_wait_ld();
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    uint32_t x[32];
-    tmem_ld32(ts + 32 * q, x);
-    tmem_wait_ld();
     if (MASK) {
 #pragma unroll
       for (int e = 0; e < 32; ++e)
-        if ((uint32_t)(first + 32 * q + e) > span) x[e] = 0xff800000u;
+        if ((uint32_t)(first + 32 * q + e) > span) x[q][e] = 0xff800000u;
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      const uint32_t* y = x + 16 * b;
+      const uint32_t* y = x[q] + 16 * b;
       float v[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(y[e]);
@@ -296,22 +289,20 @@ __device__ __forceinline__ void softmax_tile(RowState& st, uint32_t ts, uint32_t
     st.l *= alpha;
     if (has_o) {
 #pragma unroll 1
-      for (int q = 0; q < D / 32; ++q) {
-        uint32_t x[32];
-        tmem_ld32(to + 32 * q, x);
+      for (int q = 0; q < D / 16; ++q) {
+        uint32_t o[16];
+        tmem_ld_32x32b_x16(to + 16 * q, o);
         tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * alpha);
-        tmem_st32(to + 32 * q, x);
+        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+        tmem_st16(to + 16 * q, o);
       }
     }
   }
   const float base = st.ref == -INFINITY ? 0.f : st.ref;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    uint32_t x[32], p[16];
-    tmem_ld32(ts + 32 * q, x);
-    tmem_wait_ld();
+    uint32_t p[16];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const float4 f = sc[2 * q + b];
@@ -321,7 +312,7 @@ __device__ __forceinline__ void softmax_tile(RowState& st, uint32_t ts, uint32_t
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
         float y0, y1;
-        unpack2(fma2(pack2(__uint_as_float(x[16 * b + e]), __uint_as_float(x[16 * b + e + 1])),
+        unpack2(fma2(pack2(__uint_as_float(x[q][16 * b + e]), __uint_as_float(x[q][16 * b + e + 1])),
                      fk2, fv2),
                 y0, y1);
         if (MASK) {
@@ -649,10 +640,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
     }
   };
 
-  if (warp == kLoadWarp) load_role();
-  else if (warp == kMmaWarp) mma_role();
-  else if (warp >= kDequantWarp) dequant_role();
-  else softmax_role();
+  if (warp >= kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+    if (warp == kLoadWarp) load_role();
+    else if (warp == kMmaWarp) mma_role();
+  } else if (warp >= kDequantWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsDequant));
+    dequant_role();
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    softmax_role();
+  }
 
   __syncwarp();
   if (warp == kMmaWarp) {  // products still in flight (after an abort) end first
