@@ -219,6 +219,16 @@ __device__ __forceinline__ float stage_q(const AttnArgs& a, const T* p, bool val
   return fabsf(a.scale_log2) * inv;
 }
 
+// One lane of a converged warp, always the same one. Under this predicate (unlike
+// lane == 0) the compiler keeps the operands of a product in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 // Two fp32 operations in one instruction (each rounded as the scalar one).
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
   uint64_t r;
@@ -368,9 +378,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sm.tmem;
-  const uint32_t tmem_s[2] = {tmem, tmem + kTileTok};
-  const uint32_t tmem_o[2] = {tmem + 2 * kTileTok, tmem + 2 * kTileTok + D};
+  // S_t at columns 128 t, O_t at 256 + D t: the whole TMEM is allocated, from 0
   TileCursor c;
   c.x = total * blockIdx.x / W;
   c.end = total * (blockIdx.x + 1) / W;
@@ -502,14 +510,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
   auto mma_role = [&]() {
     constexpr uint32_t id_s = idesc_f16_f32(kTileRows, kTileTok);
     constexpr uint32_t id_o = idesc_f16_f32(kTileRows, D);
-    uint32_t n_q[2] = {0, 0}, n_p[2] = {0, 0};
-    auto scores = [&](int t, uint32_t slot) {
-      if (lane == 0) {
+    uint32_t n_q0 = 0, n_q1 = 0, n_p0 = 0, n_p1 = 0;
+    // One elected lane issues; a product takes 64 cycles, and its issue has to stay
+    // below that (71 measured; 83 with lane == 0 for elect_one, ~160 when the
+    // descriptors of every (tile, slot) are unrolled as constants and spill).
+    auto issue_scores = [&](int t, uint32_t slot) {
+      if (elect_one()) {
         const uint64_t qd = smem_desc(smem_addr(sm.q[t]), kTileRows * 16, 128);
         const uint64_t kd = smem_desc(smem_addr(sm.slot[slot]), 128, D * 16);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          mma_f16_ss(tmem_s[t], qd + k * (2 * kTileRows * 16 / 16), kd + k * (256 / 16), id_s,
+          mma_f16_ss(t * kTileTok, qd + k * (2 * kTileRows * 16 / 16), kd + k * (256 / 16), id_s,
                      k > 0);
         mma_commit(&sm.s_full[t]);
       }
@@ -523,32 +534,36 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
         const uint32_t ns = (2 * gi + 2) % kSlots, nu = (2 * gi + 2) / kSlots;
         if (i == 0) {
           if (!mbar_wait(&sm.slot_full[ks], ku & 1, abort)) return;
+#pragma unroll 1
           for (int t = 0; t < nt; ++t) {
-            if (!mbar_wait(&sm.q_full[t], n_q[t]++ & 1, abort)) return;
+            const uint32_t done = t ? n_q1++ : n_q0++;
+            if (!mbar_wait(&sm.q_full[t], done & 1, abort)) return;
             tc_fence_after();
-            scores(t, ks);
+            issue_scores(t, ks);
           }
-          if (lane == 0) mma_commit(&sm.slot_empty[ks]);
+          if (elect_one()) mma_commit(&sm.slot_empty[ks]);
           __syncwarp();
         }
         if (!mbar_wait(&sm.slot_full[vs], vu & 1, abort)) return;
+#pragma unroll 1
         for (int t = 0; t < nt; ++t) {
-          if (!mbar_wait(&sm.p_full[t], n_p[t]++ & 1, abort)) return;
+          const uint32_t done = t ? n_p1++ : n_p0++;
+          if (!mbar_wait(&sm.p_full[t], done & 1, abort)) return;
           tc_fence_after();
-          if (lane == 0) {
+          if (elect_one()) {
             const uint64_t vd = smem_desc(smem_addr(sm.slot[vs]), D * 16, 128);
 #pragma unroll
             for (int k = 0; k < kTileTok / 16; ++k)
-              mma_f16_ts(tmem_o[t], tmem_s[t] + 8 * k, vd + k * (2 * D * 16 / 16), id_o,
-                         i > 0 || k > 0);
+              mma_f16_ts(2 * kTileTok + t * D, t * kTileTok + 8 * k, vd + k * (2 * D * 16 / 16),
+                         id_o, i > 0 || k > 0);
             if (t == nt - 1) mma_commit(&sm.slot_empty[vs]);
             if (i + 1 == c.n) mma_commit(&sm.o_full[t]);
           }
           __syncwarp();
           if (i + 1 < c.n) {
             if (t == 0 && !mbar_wait(&sm.slot_full[ns], nu & 1, abort)) return;
-            scores(t, ns);
-            if (t == nt - 1 && lane == 0) mma_commit(&sm.slot_empty[ns]);
+            issue_scores(t, ns);
+            if (t == nt - 1 && elect_one()) mma_commit(&sm.slot_empty[ns]);
             __syncwarp();
           }
         }
@@ -559,7 +574,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
   auto softmax_role = [&]() {
     const int t = warp >> 2, row = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane 32 (warp % 4)
-    const uint32_t ts = tmem_s[t] + lanes, to = tmem_o[t] + lanes;
+    const uint32_t ts = t * kTileTok + lanes, to = 2 * kTileTok + t * D + lanes;
     uint32_t n_s = 0, n_o = 0;
     while (c.next(a, sm.pre, lane)) {
       if (t >= c.tiles(a)) {
@@ -654,14 +669,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
 
   __syncwarp();
   if (warp == kMmaWarp) {  // products still in flight (after an abort) end first
-    if (lane == 0) mma_commit(&sm.drain);
+    if (elect_one()) mma_commit(&sm.drain);
     __syncwarp();
     mbar_wait(&sm.drain, 0, abort, false);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+  if (warp == kMmaWarp) tmem_dealloc(sm.tmem, 512);
 }
 
 // Joins a unit that the shares' ends cut: the CTA column of the unit's first
