@@ -27,7 +27,7 @@ constexpr int kRawStages = 12, kSlots = 3;
 constexpr int kTileThreads = 16 * 32;  // warps 14 and 15 only complete their warpgroup
 // Registers per thread of the warpgroups (softmax twice, dequantising, products and
 // copies): together the 4 x 128 of the launch. The softmax keeps a row's 128 scores.
-constexpr int kRegsSoftmax = 184, kRegsDequant = 96, kRegsIssue = 48;
+constexpr int kRegsSoftmax = 192, kRegsDequant = 80, kRegsIssue = 48;
 static_assert(2 * kRegsSoftmax + kRegsDequant + kRegsIssue <= 4 * 128, "register shares");
 constexpr int kDequantWarp = 8, kMmaWarp = 12, kLoadWarp = 13;
 constexpr float kLazy = 8.f;  // the maximum may grow by 2^8 before O is rescaled
@@ -256,11 +256,13 @@ struct RowState {
 };
 
 // One tile of a row: scores from TMEM, weights back over the first half of their
-// columns. MASK: some row of the warp does not see all 128 tokens; the row sees
-// the columns c with (unsigned)(c + first) <= span.
-template <int D, bool MASK>
+// columns. masked: some row of the warp does not see all 128 tokens; the row sees
+// the columns c with (unsigned)(c + first) <= span. The factors of the scores are
+// kept above 0, so that a hidden score of -inf stays one.
+constexpr float kLeastFactor = 0x1p-100f;
+template <int D>
 __device__ __forceinline__ void softmax_tile(RowState& st, uint32_t ts, uint32_t to, bool has_o,
-                                             const float4* sc, float qs, int first,
+                                             const float4* sc, float qs, bool masked, int first,
                                              uint32_t span) {
   using namespace sm100;
   float top = -INFINITY;
@@ -268,13 +270,15 @@ __device__ __forceinline__ void softmax_tile(RowState& st, uint32_t ts, uint32_t
 #pragma unroll
   for (int q = 0; q < 4; ++q) tmem_ld32(ts + 32 * q, x[q]);
   tmem_wait_ld();
+  if (masked) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if (MASK) {
+    for (int q = 0; q < 4; ++q)
 #pragma unroll
       for (int e = 0; e < 32; ++e)
         if ((uint32_t)(first + 32 * q + e) > span) x[q][e] = 0xff800000u;
-    }
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const uint32_t* y = x[q] + 16 * b;
@@ -287,7 +291,7 @@ __device__ __forceinline__ void softmax_tile(RowState& st, uint32_t ts, uint32_t
         for (int z = 0; z < 4; ++z) v[z] = fmaxf(v[z], __uint_as_float(y[e + z]));
       const float bm = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
       const float4 f = sc[2 * q + b];
-      const float tm = f.y == -INFINITY || bm == -INFINITY ? -INFINITY : bm * (f.x * qs);
+      const float tm = bm * fmaxf(f.x * qs, kLeastFactor);
       st.m = fmaxf(st.m, tm);
       top = fmaxf(top, tm + f.y);
     }
@@ -316,7 +320,7 @@ __device__ __forceinline__ void softmax_tile(RowState& st, uint32_t ts, uint32_t
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const float4 f = sc[2 * q + b];
-      const float fk = f.x * qs, fv = f.y - base;
+      const float fk = fmaxf(f.x * qs, kLeastFactor), fv = f.y - base;
       const uint64_t fk2 = pack2(fk, fk), fv2 = pack2(fv, fv);
       uint64_t sum[2] = {0, 0};
 #pragma unroll
@@ -325,10 +329,6 @@ __device__ __forceinline__ void softmax_tile(RowState& st, uint32_t ts, uint32_t
         unpack2(fma2(pack2(__uint_as_float(x[q][16 * b + e]), __uint_as_float(x[q][16 * b + e + 1])),
                      fk2, fv2),
                 y0, y1);
-        if (MASK) {
-          if ((uint32_t)(first + 32 * q + 16 * b + e) > span) y0 = -INFINITY;
-          if ((uint32_t)(first + 32 * q + 16 * b + e + 1) > span) y1 = -INFINITY;
-        }
         y0 = exp2_approx(y0);
         y1 = exp2_approx(y1);
         sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(y0, y1));
@@ -609,10 +609,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
           const int first = (c.t0 + c.first + i) * kTileTok - lo;
           const bool masked = __any_sync(
               0xffffffffu, first < 0 || (uint32_t)(first + kTileTok - 1) > span);
-          if (masked)
-            softmax_tile<D, true>(st, ts, to, i > 0, sm.scale[gi & 1], qs, first, span);
-          else
-            softmax_tile<D, false>(st, ts, to, i > 0, sm.scale[gi & 1], qs, first, span);
+          softmax_tile<D>(st, ts, to, i > 0, sm.scale[gi & 1], qs, masked, first, span);
         }
         tc_fence_before();
         mbar_arrive(&sm.p_full[t]);
