@@ -211,63 +211,74 @@ __device__ __forceinline__ void load_q(const AttnArgs& a, const Seq& s, int h, i
   }
 }
 
-// One block of 16 tokens into the state. kc, vc: the lane's code words; MASK:
-// some token of the block is hidden from some row, or past the end.
-template <int D, int KIND, int NT, bool MASK>
-__device__ __forceinline__ void block_step(State<D, NT>& st, const uint4 (&kc)[D / 32],
-                                           const uint4 (&vc)[D / 32], float ks, float vs,
-                                           const uint32_t (&qf)[D / 16][NT][2],
-                                           const float (&qs)[NT][2], int t0, int len,
+// NB blocks of 16 tokens (records rec[], first tokens t0[]) into the state; two at a
+// time halve the reductions and give the warp twice the independent work. MASK:
+// some token is hidden from some row, or past the end; a null rec hides its block.
+template <int D, int KIND, int NT, int NB, bool MASK>
+__device__ __forceinline__ void block_step(State<D, NT>& st, const uint8_t* const (&rec)[NB],
+                                           const int (&t0)[NB], const uint32_t (&qf)[D / 16][NT][2],
+                                           const float (&qs)[NT][2], int len,
                                            const int (&lo)[NT][2], const int (&hi)[NT][2],
                                            int lane) {
   const int g = lane >> 2, c = lane & 3;
-  float s[NT][2][4];
+  float x[NB][NT][4], lv[NB], ivs[NB];
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+  for (int n = 0; n < NB; ++n) {
+    float s[NT][2][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[t][0][e] = s[t][1][e] = 0.f;
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    const uint32_t w[4] = {kc[i].x, kc[i].y, kc[i].z, kc[i].w};
+      for (int e = 0; e < 4; ++e) s[t][0][e] = s[t][1][e] = 0.f;
 #pragma unroll
-    for (int jj = 0; jj < 2; ++jj) {
-      uint32_t a0, a1, a2, a3;
-      code_halves<KIND>(w[2 * jj], a0, a2);
-      code_halves<KIND>(w[2 * jj + 1], a1, a3);
+    for (int i = 0; i < D / 32; ++i) {
+      const uint4 k4 = *reinterpret_cast<const uint4*>(rec[n] + 512 * i + 16 * lane);
+      const uint32_t w[4] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-        mma16816(s[t][jj], a0, a1, a2, a3, qf[2 * i + jj][t][0], qf[2 * i + jj][t][1]);
-    }
-  }
-  const float lv = __log2f(vs), ivs = __fdividef(1.f, vs);
-  uint32_t pb[NT][2];
+      for (int jj = 0; jj < 2; ++jj) {
+        uint32_t a0, a1, a2, a3;
+        code_halves<KIND>(w[2 * jj], a0, a2);
+        code_halves<KIND>(w[2 * jj + 1], a1, a3);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    float x[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[e] = (s[t][0][e] + s[t][1][e]) * (ks * qs[t][e & 1]);
-      if (MASK) {
-        const int j = t0 + g + 8 * (e >> 1);
-        if (j > hi[t][e & 1] || j < lo[t][e & 1]) x[e] = -INFINITY;
+        for (int t = 0; t < NT; ++t)
+          mma16816(s[t][jj], a0, a1, a2, a3, qf[2 * i + jj][t][0], qf[2 * i + jj][t][1]);
       }
     }
+    const float2 sc = *reinterpret_cast<const float2*>(rec[n] + 32 * D);
+    lv[n] = __log2f(sc.y);
+    ivs[n] = __fdividef(1.f, sc.y);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[n][t][e] = (s[t][0][e] + s[t][1][e]) * (sc.x * qs[t][e & 1]);
+        if (MASK) {
+          const int j = t0[n] + g + 8 * (e >> 1);
+          if (j > hi[t][e & 1] || j < lo[t][e & 1]) x[n][t][e] = -INFINITY;
+        }
+      }
+  }
+  uint32_t pb[NB][NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
     bool grew = false;
-    float alpha[2];
+    float alpha[2], ref[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      float bm = fmaxf(x[r], x[r + 2]);
-      bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 4));
-      bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 8));
-      bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 16));
-      st.m[t][r] = fmaxf(st.m[t][r], bm);
-      const float was = st.m2[t][r], now = fmaxf(was, bm + lv);
+      float top = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const float bm = fmaxf(x[n][t][r], x[n][t][r + 2]);
+        st.m[t][r] = fmaxf(st.m[t][r], bm);  // of the lane's tokens; joined at the end
+        top = fmaxf(top, bm + lv[n]);
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+      const float was = st.m2[t][r], now = fmaxf(was, top);
       grew |= now > was;
-      const float ref = now == -INFINITY ? 0.f : now;
-      alpha[r] = exp2_approx(was - ref);
+      ref[r] = now == -INFINITY ? 0.f : now;
+      alpha[r] = exp2_approx(was - ref[r]);
       st.m2[t][r] = now;
-      x[r] = exp2_approx(x[r] + (lv - ref));
-      x[r + 2] = exp2_approx(x[r + 2] + (lv - ref));
     }
     if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
@@ -280,29 +291,39 @@ __device__ __forceinline__ void block_step(State<D, NT>& st, const uint4 (&kc)[D
       st.l[t][0] *= alpha[0];
       st.l[t][1] *= alpha[1];
     }
-    st.l[t][0] = fmaf(x[0] + x[2], ivs, st.l[t][0]);
-    st.l[t][1] = fmaf(x[1] + x[3], ivs, st.l[t][1]);
-    pb[t][0] = transpose8x8(half2_bits(x[0], x[1]));
-    pb[t][1] = transpose8x8(half2_bits(x[2], x[3]));
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = exp2_approx(x[n][t][e] + (lv[n] - ref[e & 1]));
+      st.l[t][0] = fmaf(w[0] + w[2], ivs[n], st.l[t][0]);
+      st.l[t][1] = fmaf(w[1] + w[3], ivs[n], st.l[t][1]);
+      pb[n][t][0] = transpose8x8(half2_bits(w[0], w[1]));
+      pb[n][t][1] = transpose8x8(half2_bits(w[2], w[3]));
+    }
   }
-  uint32_t vmask = 0xffffffffu;
-  if (MASK && KIND == kE4m3) {
-    // places past the end may hold anything, and 0 times a NaN code is a NaN
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (t0 + 2 * c + (e & 1) + 8 * (e >> 1) >= len) vmask &= ~(0xffu << (8 * e));
-  }
+  for (int n = 0; n < NB; ++n) {
+    uint32_t vmask = 0xffffffffu;
+    if (MASK && KIND == kE4m3) {
+      // places past the end may hold anything, and 0 times a NaN code is a NaN
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    const uint32_t w[4] = {vc[i].x, vc[i].y, vc[i].z, vc[i].w};
+      for (int e = 0; e < 4; ++e)
+        if (t0[n] + 2 * c + (e & 1) + 8 * (e >> 1) >= len) vmask &= ~(0xffu << (8 * e));
+    }
 #pragma unroll
-    for (int mm = 0; mm < 2; ++mm) {
-      uint32_t a0, a1, a2, a3;
-      code_halves<KIND>(MASK ? w[2 * mm] & vmask : w[2 * mm], a0, a2);
-      code_halves<KIND>(MASK ? w[2 * mm + 1] & vmask : w[2 * mm + 1], a1, a3);
+    for (int i = 0; i < D / 32; ++i) {
+      const uint4 v4 = *reinterpret_cast<const uint4*>(rec[n] + 16 * D + 512 * i + 16 * lane);
+      const uint32_t w[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-        mma16816(st.o[2 * i + mm][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+      for (int mm = 0; mm < 2; ++mm) {
+        uint32_t a0, a1, a2, a3;
+        code_halves<KIND>(MASK ? w[2 * mm] & vmask : w[2 * mm], a0, a2);
+        code_halves<KIND>(MASK ? w[2 * mm + 1] & vmask : w[2 * mm + 1], a1, a3);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          mma16816(st.o[2 * i + mm][t], a0, a1, a2, a3, pb[n][t][0], pb[n][t][1]);
+      }
     }
   }
 }
@@ -415,15 +436,39 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
     }
     bool more = c.next(a, R, sm.pre);
     uint32_t k = 0;  // records issued
-    int i = 0;
+    int i = 0, col = 0, in_page = 0;
+    const uint8_t *page = nullptr, *rec = nullptr;
+    // The next record's address is ready before its place is: the table is read
+    // while the lane polls.
+    auto find_page = [&]() {
+      const int p = col * a.v.blocks * kBlock < c.s.len
+                        ? a.v.table[(int64_t)c.s.slot * a.v.n_cols + col] : -1;
+      if (p >= 0 && p < a.v.n_pages) {
+        page = a.v.pool + p * a.v.page_bytes() + c.unit / c.s.groups * a.v.head_bytes();
+      } else {
+        page = nullptr;
+        if (c.s.len > 0) atomicOr(&g_status, kStatusBadIndex);
+      }
+    };
+    auto find_record = [&]() {  // of block i of the piece
+      if (i == 0) {
+        const int blk = c.s.lo_blk + c.blk0;
+        col = blk / a.v.blocks;
+        in_page = blk % a.v.blocks;
+        find_page();
+      } else if (++in_page == a.v.blocks) {
+        in_page = 0;
+        ++col;
+        find_page();
+      }
+      rec = page ? page + (int64_t)in_page * rec_bytes(D) : nullptr;
+    };
+    if (more) find_record();
     unsigned long long t0 = sm100::global_ns();
     while (__any_sync(0xffffffffu, more)) {
       if (more) {
         const int st = k % S;
-        if (k < S || sm100::mbar_test(&sm.empty[lane][st], (k / S - 1) & 1)) {
-          const int blk = c.s.lo_blk + c.blk0 + i, h = c.unit / c.s.groups;
-          const uint8_t* rec =
-              blk * kBlock < c.s.len ? a.v.record(c.s.slot, blk, h) : nullptr;
+        if (k < S || sm100::mbar_poll(&sm.empty[lane][st], (k / S - 1) & 1)) {
           sm.skip[lane][st] = rec == nullptr;
           if (rec) {
             sm100::mbar_arrive_expect_tx(&sm.full[lane][st], rec_bytes(D));
@@ -436,6 +481,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
             i = 0;
             more = c.next(a, R, sm.pre);
           }
+          if (more) find_record();
           t0 = sm100::global_ns();
         } else if (*abort || sm100::global_ns() - t0 > sm100::kWaitLimitNs) {
           *abort = 1;
@@ -486,37 +532,44 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
     const int see_lo = a.window > 0 ? last - a.window + 1 : 0;
     State<D, NT> st;
     st.clear();
-    for (int i = 0; i < n; ++i, ++k) {
-      const int stage = k % S;
-      if (!sm100::mbar_wait(&sm.full[warp][stage], (k / S) & 1, abort)) return;
-      const uint8_t* rec = sm.ring[warp][stage];
-      uint4 kc[D / 32], vc[D / 32];
-#pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        kc[j] = *reinterpret_cast<const uint4*>(rec + 512 * j + 16 * lane);
-        vc[j] = *reinterpret_cast<const uint4*>(rec + 16 * D + 512 * j + 16 * lane);
-      }
-      const float2 sc = *reinterpret_cast<const float2*>(rec + 32 * D);
-      const bool skip = sm.skip[warp][stage];
-      __syncwarp();
-      if (lane == 0) sm100::mbar_arrive(&sm.empty[warp][stage]);
-      if (skip) continue;
+    auto visible = [&](int t0) { return t0 >= see_lo && t0 + kBlock - 1 <= see_hi; };
+    for (int i = 0; i < n;) {
       const int t0 = (s.lo_blk + cur.blk0 + i) * kBlock;
-      if (t0 >= see_lo && t0 + kBlock - 1 <= see_hi)
-        block_step<D, KIND, NT, false>(st, kc, vc, sc.x, sc.y, qf, qs, t0, s.len, lo, hi, lane);
-      else
-        block_step<D, KIND, NT, true>(st, kc, vc, sc.x, sc.y, qf, qs, t0, s.len, lo, hi, lane);
+      const int s0 = k % S, s1 = (k + 1) % S;
+      if (!sm100::mbar_wait(&sm.full[warp][s0], (k / S) & 1, abort)) return;
+      const uint8_t* r0 = sm.ring[warp][s0];
+      bool pair = i + 1 < n;
+      if (pair) {
+        if (!sm100::mbar_wait(&sm.full[warp][s1], ((k + 1) / S) & 1, abort)) return;
+        pair = !sm.skip[warp][s0] && !sm.skip[warp][s1];
+      }
+      if (pair) {
+        const uint8_t* const rec[2] = {r0, sm.ring[warp][s1]};
+        const int at[2] = {t0, t0 + kBlock};
+        if (visible(t0) && visible(t0 + kBlock))
+          block_step<D, KIND, NT, 2, false>(st, rec, at, qf, qs, s.len, lo, hi, lane);
+        else
+          block_step<D, KIND, NT, 2, true>(st, rec, at, qf, qs, s.len, lo, hi, lane);
+      } else if (!sm.skip[warp][s0]) {
+        const uint8_t* const rec[1] = {r0};
+        const int at[1] = {t0};
+        block_step<D, KIND, NT, 1, true>(st, rec, at, qf, qs, s.len, lo, hi, lane);
+      }
+      const int used = pair ? 2 : 1;
+      __syncwarp();
+      if (lane < used) sm100::mbar_arrive(&sm.empty[warp][lane ? s1 : s0]);
+      i += used;
+      k += used;
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float l = st.l[t][r];
-        l += __shfl_xor_sync(0xffffffffu, l, 4);
-        l += __shfl_xor_sync(0xffffffffu, l, 8);
-        l += __shfl_xor_sync(0xffffffffu, l, 16);
-        st.l[t][r] = l;
-      }
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int o = 4; o <= 16; o *= 2) {
+          st.l[t][r] += __shfl_xor_sync(0xffffffffu, st.l[t][r], o);
+          st.m[t][r] = fmaxf(st.m[t][r], __shfl_xor_sync(0xffffffffu, st.m[t][r], o));
+        }
     const bool whole = n == s.n_blk;  // the whole unit: its rows are done
     float* p = a.part + (2 * w + (cur.blk0 == 0)) * part_floats(D, NT);
 #pragma unroll
