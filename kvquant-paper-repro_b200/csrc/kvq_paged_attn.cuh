@@ -81,24 +81,39 @@ struct Seq {
   int slot, len, n, lo_blk, n_blk, groups;
   int64_t r0;
 };
-__device__ __forceinline__ Seq load_seq(const AttnArgs& a, int64_t b, int R) {
+// The parts of a Seq that come from memory, kept in shared memory by kernels that
+// need a sequence more than once (calls of up to kSeqCache sequences).
+constexpr int kSeqCache = 1024;
+__device__ __forceinline__ Seq make_seq(const AttnArgs& a, int slot, int len, int n, int64_t r0,
+                                        int R) {
   Seq s;
-  int64_t r1;
-  a.v.rows(b, s.r0, r1);
-  s.n = (int)(r1 - s.r0);
-  if (s.n > a.max_new) {
-    atomicOr(&g_status, kStatusBadIndex);
-    s.n = 0;
-  }
-  s.slot = a.v.slot(b);
-  s.len = s.slot < 0 ? 0 : a.v.length(s.slot);
-  const int lo = a.window > 0 ? max(0, s.len - s.n - a.window + 1) : 0;
+  s.slot = slot;
+  s.len = len;
+  s.n = n;
+  s.r0 = r0;
+  const int lo = a.window > 0 ? max(0, len - n - a.window + 1) : 0;
   s.lo_blk = lo / kBlock;
   // an empty sequence still has a (wholly masked) block, which writes its rows
-  s.n_blk = max(1, (s.len + kBlock - 1) / kBlock - s.lo_blk);
-  s.groups = (int)(((int64_t)s.n * a.group + R - 1) / R);
-  if (s.n == 0) s.n_blk = 0;
+  s.n_blk = n == 0 ? 0 : max(1, (len + kBlock - 1) / kBlock - s.lo_blk);
+  s.groups = (int)(((int64_t)n * a.group + R - 1) / R);
   return s;
+}
+
+__device__ __forceinline__ Seq load_seq(const AttnArgs& a, int64_t b, int R,
+                                        const int4* cache = nullptr) {
+  if (cache) {
+    const int4 c = cache[b];
+    return make_seq(a, c.x, c.y, c.z, c.w, R);
+  }
+  int64_t r0, r1;
+  a.v.rows(b, r0, r1);
+  int n = (int)(r1 - r0);
+  if (n > a.max_new) {
+    atomicOr(&g_status, kStatusBadIndex);
+    n = 0;
+  }
+  const int slot = a.v.slot(b);
+  return make_seq(a, slot, slot < 0 ? 0 : a.v.length(slot), n, r0, R);
 }
 
 // Work is a flat sequence of 16-token blocks over (sequence, head, row group),
@@ -106,7 +121,7 @@ __device__ __forceinline__ Seq load_seq(const AttnArgs& a, int64_t b, int R) {
 // = blocks of the sequences before b, per head. Block-wide; pre has B + 1 places.
 template <int THREADS>
 __device__ __forceinline__ int64_t block_prefix(const AttnArgs& a, int R, int64_t* pre,
-                                                int64_t* sums) {
+                                                int64_t* sums, int4* cache = nullptr) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   int64_t base = 0;
   for (int64_t b0 = 0; b0 < a.v.B; b0 += THREADS) {
@@ -115,6 +130,7 @@ __device__ __forceinline__ int64_t block_prefix(const AttnArgs& a, int R, int64_
     if (b < a.v.B) {
       const Seq s = load_seq(a, b, R);
       x = (int64_t)s.n_blk * s.groups;
+      if (cache) cache[b] = make_int4(s.slot, s.len, s.n, (int)s.r0);
     }
     int64_t incl = x;
 #pragma unroll
@@ -372,7 +388,7 @@ struct AttnSmem {
   int skip[kAttnWarps][Ring<D>::kStages];
   int abort;
   int64_t sums[32];
-  int64_t pre[1];  // B + 1
+  alignas(16) int64_t pre[2];  // B + 1, then the sequences (16 bytes each)
 };
 
 // Where a worker stands in its share of the blocks.
@@ -382,7 +398,7 @@ struct Cursor {
   Seq s;
   int unit, blk0, n;
   // The next piece (blocks of one unit); false when the share is done.
-  __device__ bool next(const AttnArgs& a, int R, const int64_t* pre) {
+  __device__ bool next(const AttnArgs& a, int R, const int64_t* pre, const int4* cache) {
     if (x >= end) return false;
     int64_t lo = 0, hi = a.v.B;  // largest b with pre[b] * heads <= x
     while (hi - lo > 1) {
@@ -391,7 +407,7 @@ struct Cursor {
       else hi = mid;
     }
     b = lo;
-    s = load_seq(a, b, R);
+    s = load_seq(a, b, R, cache);
     const int64_t rem = x - pre[b] * a.v.heads;
     unit = (int)(rem / s.n_blk);
     blk0 = (int)(rem % s.n_blk);
@@ -420,7 +436,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
   sm100::fence_mbar_init();
   wait_previous();
   let_next_start();
-  const int64_t total = block_prefix<kAttnThreads>(a, R, sm.pre, sm.sums);  // syncs the block
+  int4* cache =
+      a.v.B <= kSeqCache ? reinterpret_cast<int4*>(sm.pre + ((a.v.B + 2) & ~1ll)) : nullptr;
+  const int64_t total =
+      block_prefix<kAttnThreads>(a, R, sm.pre, sm.sums, cache);  // syncs the block
   if (total == 0) return;
   const int64_t W = workers_of(a, total);
   volatile int* abort = &sm.abort;
@@ -434,7 +453,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
       c.x = total * w / W;
       c.end = total * (w + 1) / W;
     }
-    bool more = c.next(a, R, sm.pre);
+    bool more = c.next(a, R, sm.pre, cache);
     uint32_t k = 0;  // records issued
     int i = 0, col = 0, in_page = 0;
     const uint8_t *page = nullptr, *rec = nullptr;
@@ -479,7 +498,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
           ++k;
           if (++i == c.n) {
             i = 0;
-            more = c.next(a, R, sm.pre);
+            more = c.next(a, R, sm.pre, cache);
           }
           if (more) find_record();
           t0 = sm100::global_ns();
@@ -510,7 +529,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
   cur.end = total * (w + 1) / W;
   const int g = lane >> 2, c = lane & 3;
   uint32_t k = 0;
-  while (cur.next(a, R, sm.pre)) {
+  while (cur.next(a, R, sm.pre, cache)) {
     const Seq& s = cur.s;
     const int n = cur.n, h = cur.unit / s.groups, row0 = cur.unit % s.groups * R;
     uint32_t qf[D / 16][NT][2];
@@ -603,83 +622,99 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
   }
 }
 
-// Joins the pieces of the units that several workers share, in the workers'
-// order: one CTA per (unit, row). The pieces' weights come first, 256 at a time,
-// then G = 256 / D groups of threads add every G-th piece.
-constexpr int kJoinThreads = 256;
+// Joins the pieces of the units that several workers share, in a fixed order. A
+// CTA takes `rows` of the unit_rows rows that a unit can have, 8 / rows warps each
+// (few units have many pieces); a lane adds D / 32 channels of its warp's pieces,
+// 32 weights at a time.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
 
 template <int D, int NT, typename T>
-__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttnArgs a) {
-  constexpr int R = 8 * NT, G = kJoinThreads / D;
+__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttnArgs a, int unit_rows, int rows) {
+  constexpr int R = 8 * NT, C = D / 32;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   int64_t* pre = reinterpret_cast<int64_t*>(smem_raw);
   __shared__ int64_t sums[32];
-  __shared__ float weight[kJoinThreads], red[3][kJoinThreads / 32], acc[G][D];
+  __shared__ float acc[kJoinWarps][D], sum[kJoinWarps];
   // lengths and rows are not written by the kernel before: read ahead of the wait
   const int64_t total = block_prefix<kJoinThreads>(a, R, pre, sums);
   const int64_t W = workers_of(a, total);
   const int64_t b = blockIdx.y;
   const Seq s = load_seq(a, b, R);
-  const int unit = blockIdx.x / R, r = blockIdx.x % R;
+  const int split = kJoinWarps / rows, wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per_unit = unit_rows / rows;
+  const int first = (int)(blockIdx.x % per_unit) * rows, unit = blockIdx.x / per_unit;
+  const int r = first + wid / split, part = wid % split;
+  const int h = unit / max(1, s.groups), row = unit % max(1, s.groups) * R + r;
+  // worker w holds the blocks [total w / W, total (w + 1) / W)
+  const int64_t x0 = pre[b] * a.v.heads + (int64_t)unit * s.n_blk, x1 = x0 + s.n_blk;
+  const bool here = total > 0 && unit < s.groups * a.v.heads && row < s.n * a.group;
+  const int64_t w0 = here ? ((x0 + 1) * W - 1) / total : 0;
+  const int64_t w1 = here ? (x1 * W - 1) / total : 0;
   wait_previous();
   let_next_start();
-  if (total == 0 || unit >= s.groups * a.v.heads) return;
-  const int h = unit / s.groups, row = unit % s.groups * R + r;
-  if (row >= s.n * a.group) return;
-  const int64_t x0 = pre[b] * a.v.heads + (int64_t)unit * s.n_blk, x1 = x0 + s.n_blk;
-  // worker w holds the blocks [total w / W, total (w + 1) / W)
-  const int64_t w0 = ((x0 + 1) * W - 1) / total, w1 = (x1 * W - 1) / total;
-  if (w0 == w1) return;
-  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, d = tid % D, grp = tid / D;
-  const int n = (int)(w1 - w0) + 1;
+  const int n = w1 > w0 ? (int)(w1 - w0) + 1 : 0;  // the row's pieces (0: nothing to join)
+  float m = -INFINITY, m2 = -INFINITY, l = 0.f, o[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) o[i] = 0.f;
   auto piece = [&](int i) {  // the first piece is its worker's last, the others their first
     return a.part + (2 * (w0 + i) + (i == 0)) * part_floats(D, NT);
   };
-  auto block_max = [&](float x, float* buf) {
-    x = warp_max(x);
-    if (lane == 0) buf[wid] = x;
-    __syncthreads();
-    x = buf[0];
-#pragma unroll
-    for (int i = 1; i < kJoinThreads / 32; ++i) x = fmaxf(x, buf[i]);
-    return x;
-  };
-  float m = -INFINITY, m2 = -INFINITY, l = 0.f, o = 0.f;
-  for (int i = tid; i < n; i += kJoinThreads) {
+  for (int i = lane; i < n; i += 32) {
     const float4 q = *reinterpret_cast<const float4*>(piece(i) + R * D + 4 * r);
     m2 = fmaxf(m2, q.x);
     m = fmaxf(m, q.z);
   }
-  m2 = block_max(m2, red[0]);
-  m = block_max(m, red[1]);
+  m2 = warp_max(m2);
+  m = warp_max(m);
   const float ref = m2 == -INFINITY ? 0.f : m2;
-  for (int i0 = 0; i0 < n; i0 += kJoinThreads) {
-    __syncthreads();
-    if (i0 + tid < n) {
-      const float4 q = *reinterpret_cast<const float4*>(piece(i0 + tid) + R * D + 4 * r);
-      const float f = exp2_approx(q.x - ref);
-      weight[tid] = f;
+  for (int i0 = part; i0 < n; i0 += 32 * split) {  // pieces i0, i0 + split, ..
+    float f = 0.f;
+    const int mine = i0 + split * lane;
+    if (mine < n) {
+      const float4 q = *reinterpret_cast<const float4*>(piece(mine) + R * D + 4 * r);
+      f = exp2_approx(q.x - ref);
       l = fmaf(q.y, f, l);
     }
-    __syncthreads();
-    const int k = min(kJoinThreads, n - i0);
+    const int k = min(32, (n - i0 + split - 1) / split);
 #pragma unroll 8
-    for (int i = grp; i < k; i += G) o = fmaf(piece(i0 + i)[r * D + d], weight[i], o);
+    for (int i = 0; i < k; ++i) {
+      const float w = __shfl_sync(0xffffffffu, f, i);
+      const float* p = piece(i0 + split * i) + r * D + C * lane;
+      float x[C];
+      if constexpr (C == 4) {
+        const float4 y = *reinterpret_cast<const float4*>(p);
+        x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
+      } else {
+        const float2 y = *reinterpret_cast<const float2*>(p);
+        x[0] = y.x; x[1] = y.y;
+      }
+#pragma unroll
+      for (int e = 0; e < C; ++e) o[e] = fmaf(x[e], w, o[e]);
+    }
   }
   l = warp_sum(l);
-  if (lane == 0) red[2][wid] = l;
-  acc[grp][d] = o;
-  __syncthreads();
-  if (grp) return;
-  l = 0.f;
+  if (split > 1) {
 #pragma unroll
-  for (int i = 0; i < kJoinThreads / 32; ++i) l += red[2][i];
+    for (int e = 0; e < C; ++e) acc[wid][C * lane + e] = o[e];
+    if (lane == 0) sum[wid] = l;
+    __syncthreads();
+    if (part) return;
+    for (int i = 1; i < split; ++i) {
 #pragma unroll
-  for (int i = 1; i < G; ++i) o += acc[i][d];
+      for (int e = 0; e < C; ++e) o[e] += acc[wid + i][C * lane + e];
+      l += sum[wid + i];
+    }
+  }
+  if (n == 0) return;
   const int64_t at = (s.r0 + row / a.group) * ((int64_t)a.v.heads * a.group) + h * a.group +
                      row % a.group;
-  ((T*)a.out)[at * D + d] = from_float<T>(l == 0.f ? 0.f : o * __fdiv_rn(1.f, l));
-  if (a.ml && d == 0) a.ml[at] = row_stats(m, m2, l);
+  const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+  T* out = (T*)a.out + at * D + C * lane;
+#pragma unroll
+  for (int e = 0; e < C; e += 2)
+    *reinterpret_cast<uint32_t*>(out + e) =
+        l == 0.f ? 0u : from_float2<T>(o[e] * inv, o[e + 1] * inv);
+  if (a.ml && lane == 0) a.ml[at] = row_stats(m, m2, l);
 }
 
 // Rows of a call's largest sequence: 8-row tiles where one or two are enough,
@@ -709,16 +744,27 @@ template <int D, int KIND, int NT, typename T>
 static int launch_attend(AttnArgs a, cudaStream_t st) {
   const int64_t groups = ((int64_t)a.max_new * a.group + 8 * NT - 1) / (8 * NT);
   a.n_workers = kSms * kAttnWarps;
-  const int smem = (int)(sizeof(AttnSmem<D>) + a.v.B * sizeof(int64_t));
+  const int64_t cached = a.v.B <= kSeqCache ? a.v.B : 0;
+  const int smem = (int)(sizeof(AttnSmem<D>) + a.v.B * sizeof(int64_t) + cached * sizeof(int4));
+  static_assert(sizeof(AttnSmem<D>) + kMaxSeqs * sizeof(int64_t) <= 227 * 1024 &&
+                    kSeqCache * (sizeof(int64_t) + sizeof(int4)) <= kMaxSeqs * sizeof(int64_t),
+                "shared memory");
   // once per device would do; the call is cheap and keeps no state
   cudaFuncSetAttribute(attend_kernel<D, KIND, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                       (int)(sizeof(AttnSmem<D>) + kMaxSeqs * sizeof(int64_t)));
+                       227 * 1024);
   int rc = launch_next("paged_attention", attend_kernel<D, KIND, NT, T>, dim3(kSms), kAttnThreads,
                        smem, st, a);
   if (rc) return rc;
-  const dim3 grid((unsigned)(groups * a.v.heads * 8 * NT), (unsigned)a.v.B);
+  // rows per CTA: as few CTAs as keep the SMs busy, for they start beside the last
+  // attention CTAs
+  int unit_rows = 1;
+  while (unit_rows < 8 * NT && unit_rows < (int64_t)a.max_new * a.group) unit_rows *= 2;
+  const int64_t units = groups * a.v.heads * a.v.B;
+  int rows = unit_rows < 8 ? unit_rows : 8;
+  while (rows > 1 && units * (unit_rows / rows) * 2 <= kSms) rows /= 2;
+  const dim3 grid((unsigned)(groups * a.v.heads * (unit_rows / rows)), (unsigned)a.v.B);
   return launch_next("paged_attention (join)", attend_join_kernel<D, NT, T>, grid, kJoinThreads,
-                     (int)((a.v.B + 1) * sizeof(int64_t)), st, a);
+                     (int)((a.v.B + 1) * sizeof(int64_t)), st, a, unit_rows, rows);
 }
 
 }  // namespace paged
