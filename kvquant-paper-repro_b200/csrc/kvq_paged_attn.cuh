@@ -14,6 +14,8 @@
 // power of two; products and sums are fp32. The only roundings to fewer bits
 // are w_j (fp16, relative 2^-12, or 2^-25 of the largest) and the output.
 #pragma once
+#include <atomic>
+
 #include "kvq_paged.cuh"
 
 namespace kvq {
@@ -117,8 +119,12 @@ __device__ __forceinline__ Seq load_seq(const AttnArgs& a, int64_t b, int R,
 }
 
 // Work is a flat sequence of 16-token blocks over (sequence, head, row group),
-// and worker w of W takes an equal share of it, whatever the lengths are. pre[b]
-// = blocks of the sequences before b, per head. Block-wide; pre has B + 1 places.
+// and worker w of W takes an equal share of it, whatever the lengths are. Each
+// unit counts kUnitCost blocks more than it has, its first places: starting and
+// ending a unit takes a warp about that long (2 us against 0.84 us a block), and
+// workers with many short sequences ended 6 us after the others without it.
+// pre[b] = places of the sequences before b, per head. Block-wide; pre has B + 1.
+constexpr int kUnitCost = 2;
 template <int THREADS>
 __device__ __forceinline__ int64_t block_prefix(const AttnArgs& a, int R, int64_t* pre,
                                                 int64_t* sums, int4* cache = nullptr) {
@@ -129,7 +135,7 @@ __device__ __forceinline__ int64_t block_prefix(const AttnArgs& a, int R, int64_
     int64_t x = 0;
     if (b < a.v.B) {
       const Seq s = load_seq(a, b, R);
-      x = (int64_t)s.n_blk * s.groups;
+      x = (int64_t)(s.n_blk + kUnitCost) * s.groups;
       if (cache) cache[b] = make_int4(s.slot, s.len, s.n, (int)s.r0);
     }
     int64_t incl = x;
@@ -399,7 +405,11 @@ struct Cursor {
   int unit, blk0, n;
   // The next piece (blocks of one unit); false when the share is done.
   __device__ bool next(const AttnArgs& a, int R, const int64_t* pre, const int4* cache) {
-    if (x >= end) return false;
+    n = 0;
+    while (x < end && n == 0) find(a, R, pre, cache);
+    return n > 0;
+  }
+  __device__ void find(const AttnArgs& a, int R, const int64_t* pre, const int4* cache) {
     int64_t lo = 0, hi = a.v.B;  // largest b with pre[b] * heads <= x
     while (hi - lo > 1) {
       const int64_t mid = (lo + hi) >> 1;
@@ -408,12 +418,13 @@ struct Cursor {
     }
     b = lo;
     s = load_seq(a, b, R, cache);
+    const int len = s.n_blk + kUnitCost;
     const int64_t rem = x - pre[b] * a.v.heads;
-    unit = (int)(rem / s.n_blk);
-    blk0 = (int)(rem % s.n_blk);
-    n = (int)min((int64_t)(s.n_blk - blk0), end - x);
-    x += n;
-    return true;
+    unit = (int)(rem / len);
+    const int at = (int)(rem % len), to = (int)min((int64_t)len, at + (end - x));
+    x += to - at;
+    blk0 = max(at - kUnitCost, 0);
+    n = max(to - kUnitCost, 0) - blk0;
   }
 };
 
@@ -435,7 +446,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
   if (threadIdx.x == 0) sm.abort = 0;
   sm100::fence_mbar_init();
   wait_previous();
-  let_next_start();
+  let_next_start();  // only now: the join reads lengths before its own wait
   int4* cache =
       a.v.B <= kSeqCache ? reinterpret_cast<int4*>(sm.pre + ((a.v.B + 2) & ~1ll)) : nullptr;
   const int64_t total =
@@ -623,10 +634,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
 }
 
 // Joins the pieces of the units that several workers share, in a fixed order. A
-// CTA takes `rows` of the unit_rows rows that a unit can have, 8 / rows warps each
+// CTA takes `rows` of the unit_rows rows that a unit can have, 4 / rows warps each
 // (few units have many pieces); a lane adds D / 32 channels of its warp's pieces,
-// 32 weights at a time.
-constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+// 32 weights at a time. Four warps fit beside an attention CTA (eight do not: the
+// registers), so the CTAs are there, lengths read, when the last piece is written.
+constexpr int kJoinThreads = 128, kJoinWarps = kJoinThreads / 32;
 
 template <int D, int NT, typename T>
 __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttnArgs a, int unit_rows, int rows) {
@@ -635,7 +647,9 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttnArgs a, i
   int64_t* pre = reinterpret_cast<int64_t*>(smem_raw);
   __shared__ int64_t sums[32];
   __shared__ float acc[kJoinWarps][D], sum[kJoinWarps];
-  // lengths and rows are not written by the kernel before: read ahead of the wait
+  let_next_start();
+  // the attention kernel has waited for whatever writes lengths and rows, so they are
+  // read ahead of the wait for it
   const int64_t total = block_prefix<kJoinThreads>(a, R, pre, sums);
   const int64_t W = workers_of(a, total);
   const int64_t b = blockIdx.y;
@@ -645,13 +659,13 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttnArgs a, i
   const int first = (int)(blockIdx.x % per_unit) * rows, unit = blockIdx.x / per_unit;
   const int r = first + wid / split, part = wid % split;
   const int h = unit / max(1, s.groups), row = unit % max(1, s.groups) * R + r;
-  // worker w holds the blocks [total w / W, total (w + 1) / W)
-  const int64_t x0 = pre[b] * a.v.heads + (int64_t)unit * s.n_blk, x1 = x0 + s.n_blk;
+  // worker w holds the places [total w / W, total (w + 1) / W)
+  const int64_t x1 = pre[b] * a.v.heads + (int64_t)(unit + 1) * (s.n_blk + kUnitCost);
+  const int64_t x0 = x1 - s.n_blk;
   const bool here = total > 0 && unit < s.groups * a.v.heads && row < s.n * a.group;
   const int64_t w0 = here ? ((x0 + 1) * W - 1) / total : 0;
   const int64_t w1 = here ? (x1 * W - 1) / total : 0;
   wait_previous();
-  let_next_start();
   const int n = w1 > w0 ? (int)(w1 - w0) + 1 : 0;  // the row's pieces (0: nothing to join)
   float m = -INFINITY, m2 = -INFINITY, l = 0.f, o[C];
 #pragma unroll
@@ -659,10 +673,17 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttnArgs a, i
   auto piece = [&](int i) {  // the first piece is its worker's last, the others their first
     return a.part + (2 * (w0 + i) + (i == 0)) * part_floats(D, NT);
   };
-  for (int i = lane; i < n; i += 32) {
-    const float4 q = *reinterpret_cast<const float4*>(piece(i) + R * D + 4 * r);
-    m2 = fmaxf(m2, q.x);
-    m = fmaxf(m, q.z);
+  float4 own = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);  // of piece part + split * lane
+  if (part + split * lane < n)
+    own = *reinterpret_cast<const float4*>(piece(part + split * lane) + R * D + 4 * r);
+  m2 = own.x;
+  m = own.z;
+  if (split > 1 || n > 32) {
+    for (int i = lane; i < n; i += 32) {
+      const float4 q = *reinterpret_cast<const float4*>(piece(i) + R * D + 4 * r);
+      m2 = fmaxf(m2, q.x);
+      m = fmaxf(m, q.z);
+    }
   }
   m2 = warp_max(m2);
   m = warp_max(m);
@@ -671,7 +692,8 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttnArgs a, i
     float f = 0.f;
     const int mine = i0 + split * lane;
     if (mine < n) {
-      const float4 q = *reinterpret_cast<const float4*>(piece(mine) + R * D + 4 * r);
+      const float4 q =
+          i0 == part ? own : *reinterpret_cast<const float4*>(piece(mine) + R * D + 4 * r);
       f = exp2_approx(q.x - ref);
       l = fmaf(q.y, f, l);
     }
@@ -723,6 +745,19 @@ inline int row_tiles(int64_t max_new, int64_t group) {
   return max_new * group <= 8 ? 1 : max_new * group <= 16 ? 2 : 0;
 }
 
+// Allows `kernel` `bytes` of dynamic shared memory on the current device; `done` is
+// the kernel's own set of the devices where that has been said already.
+template <typename K>
+static void allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) ==
+      cudaSuccess)
+    done.fetch_or(bit, std::memory_order_relaxed);
+}
+
 template <typename... Params, typename... Args>
 static int launch_next(const char* what, void (*kernel)(Params...), dim3 grid, int threads,
                        int smem, cudaStream_t st, const Args&... args) {
@@ -749,9 +784,8 @@ static int launch_attend(AttnArgs a, cudaStream_t st) {
   static_assert(sizeof(AttnSmem<D>) + kMaxSeqs * sizeof(int64_t) <= 227 * 1024 &&
                     kSeqCache * (sizeof(int64_t) + sizeof(int4)) <= kMaxSeqs * sizeof(int64_t),
                 "shared memory");
-  // once per device would do; the call is cheap and keeps no state
-  cudaFuncSetAttribute(attend_kernel<D, KIND, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                       227 * 1024);
+  static std::atomic<uint64_t> done{0};
+  allow_smem(attend_kernel<D, KIND, NT, T>, 227 * 1024, done);
   int rc = launch_next("paged_attention", attend_kernel<D, KIND, NT, T>, dim3(kSms), kAttnThreads,
                        smem, st, a);
   if (rc) return rc;
@@ -760,7 +794,7 @@ static int launch_attend(AttnArgs a, cudaStream_t st) {
   int unit_rows = 1;
   while (unit_rows < 8 * NT && unit_rows < (int64_t)a.max_new * a.group) unit_rows *= 2;
   const int64_t units = groups * a.v.heads * a.v.B;
-  int rows = unit_rows < 8 ? unit_rows : 8;
+  int rows = unit_rows < kJoinWarps ? unit_rows : kJoinWarps;
   while (rows > 1 && units * (unit_rows / rows) * 2 <= kSms) rows /= 2;
   const dim3 grid((unsigned)(groups * a.v.heads * (unit_rows / rows)), (unsigned)a.v.B);
   return launch_next("paged_attention (join)", attend_join_kernel<D, NT, T>, grid, kJoinThreads,

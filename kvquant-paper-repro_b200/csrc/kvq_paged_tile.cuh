@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
     fence_mbar_init();
   }
   wait_previous();
-  let_next_start();
+  let_next_start();  // only now: the join reads lengths before its own wait
   const int64_t total = tile_prefix<kTileThreads>(a, sm.pre, sm.sums);  // syncs the block
   const int64_t W = tile_workers(total);
   if (total == 0 || blockIdx.x >= W) return;
@@ -678,17 +678,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
 
 // Joins a unit that the shares' ends cut: the CTA column of the unit's first
 // inner cut adds its pieces in order, 32 rows per CTA.
-constexpr int kTileJoinRows = 32;
+constexpr int kTileJoinRows = 32, kTileJoinThreads = 256;
 
 template <int D, typename T>
-__global__ void __launch_bounds__(kJoinThreads) tile_join_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(kTileJoinThreads) tile_join_kernel(AttnArgs a) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   int32_t* pre = reinterpret_cast<int32_t*>(smem_raw);
   __shared__ int64_t sums[32];
-  const int64_t total = tile_prefix<kJoinThreads>(a, pre, sums);
+  let_next_start();
+  const int64_t total = tile_prefix<kTileJoinThreads>(a, pre, sums);
   // every CTA waits, or a later launch could pass the attention kernel
   wait_previous();
-  let_next_start();
   const int64_t W = tile_workers(total), cut = blockIdx.x + 1;
   if (total == 0 || cut >= W) return;
   TileCursor c;
@@ -698,7 +698,7 @@ __global__ void __launch_bounds__(kJoinThreads) tile_join_kernel(AttnArgs a) {
   c.next(a, pre, threadIdx.x & 31);
   const int64_t start = x - c.first, end = start + c.n_unit;
   if (c.first == 0 || total * (cut - 1) / W > start) return;
-  constexpr int G = kJoinThreads / D, F = kUnitRows * (D + 4);
+  constexpr int G = kTileJoinThreads / D, F = kUnitRows * (D + 4);
   const int d = threadIdx.x % D;
   for (int i = threadIdx.x / D; i < kTileJoinRows; i += G) {
     const int ur = blockIdx.y * kTileJoinRows + i, r = c.row0 + ur;
@@ -724,13 +724,14 @@ __global__ void __launch_bounds__(kJoinThreads) tile_join_kernel(AttnArgs a) {
 template <int D, int KIND, typename T>
 static int launch_attend_tile(AttnArgs a, cudaStream_t st) {
   const int smem = (int)(sizeof(TileSmem<D>) + a.v.B * sizeof(int32_t));
-  cudaFuncSetAttribute(attend_tile_kernel<D, KIND, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                       (int)(sizeof(TileSmem<D>) + kMaxSeqs * sizeof(int32_t)));
+  static_assert(sizeof(TileSmem<D>) + kMaxSeqs * sizeof(int32_t) <= 227 * 1024, "shared memory");
+  static std::atomic<uint64_t> done{0};
+  allow_smem(attend_tile_kernel<D, KIND, T>, 227 * 1024, done);
   int rc = launch_next("paged_attention (tiles)", attend_tile_kernel<D, KIND, T>, dim3(kSms),
                        kTileThreads, smem, st, a);
   if (rc) return rc;
   return launch_next("paged_attention (tile join)", tile_join_kernel<D, T>,
-                     dim3(kSms - 1, kUnitRows / kTileJoinRows), kJoinThreads,
+                     dim3(kSms - 1, kUnitRows / kTileJoinRows), kTileJoinThreads,
                      (int)((a.v.B + 1) * sizeof(int32_t)), st, a);
 }
 

@@ -25,8 +25,6 @@ get_cuda_ops().check_status().
 """
 from __future__ import annotations
 
-import math
-
 import torch
 
 from .cuda_ops import _check, _ptr, get_cuda_ops
@@ -37,15 +35,20 @@ KINDS = {"int8": 0, "e4m3": 1}
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
-def _launch(fn, lib, dev, *args) -> None:
-    """fn(*args, current stream of dev) with dev current. These calls take microseconds on
-    the GPU, so the device is switched only when it has to be."""
-    i = dev.index
-    if i == torch.cuda.current_device():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+# Calls take microseconds on the GPU, so the checks below use the cheapest form of each
+# question (device numbers, identity of dtypes) and the device is switched only when it
+# has to be.
+_current_device = torch.cuda.current_device
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _launch(fn, lib, dev: int, *args) -> None:
+    """fn(*args, current stream of device dev) with dev current."""
+    if dev == _current_device():
+        rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+            rc = fn(*args, _raw_stream(dev))
     if rc:
         _check(rc, lib)
 
@@ -59,58 +62,57 @@ def pool_shape(n_pages: int, heads: int, head_dim: int, page_tokens: int) -> tup
     return n_pages, heads, page_tokens // BLOCK_TOKENS, record_bytes(head_dim)
 
 
-def _kind(what: str, kind: str) -> int:
-    if kind not in KINDS:
-        raise RuntimeError(f"{what}: kind must be one of {sorted(KINDS)}, got {kind!r}")
-    return KINDS[kind]
-
-
-def _int32(what: str, name: str, t, device, shape=None):
+def _int32(what: str, name: str, t, dev: int, n: int | None = None):
+    """Pointer of a contiguous int32 tensor on device dev (with n elements), or None."""
     if t is None:
         return None
-    if (t.dtype != torch.int32 or t.device != device or not t.is_contiguous()
-            or (shape is not None and tuple(t.shape) != shape)):
-        want = "" if shape is None else f" {shape}"
-        raise RuntimeError(f"{what}: {name} must be contiguous int32{want} on {device}")
+    if (t.dtype is not torch.int32 or t.get_device() != dev or not t.is_contiguous()
+            or (n is not None and t.numel() != n)):
+        size = "" if n is None else f" with {n} elements"
+        raise RuntimeError(f"{what}: {name} must be contiguous int32{size} on cuda:{dev}")
     return t.data_ptr()
 
 
-def _cache_args(what: str, pool, kind, table, lengths, slots, indptr, total):
-    """The arguments that describe a layer's cache and a call's sequences; and B."""
-    if not pool.is_cuda:
+def _cache_args(what: str, pool, kind, table, lengths, slots, indptr):
+    """The arguments that describe a layer's cache and a call's sequences, the latter's
+    number, KV heads, channels and the device."""
+    dev = pool.get_device()
+    if dev < 0:
         raise RuntimeError(f"{what}: kvquant_b200 runs on CUDA tensors only")
-    if pool.dtype != torch.uint8 or pool.dim() != 4 or not pool.is_contiguous():
+    if pool.dtype is not torch.uint8 or pool.dim() != 4 or not pool.is_contiguous():
         raise RuntimeError(f"{what}: pool must be contiguous uint8 [pages, heads, blocks, record]")
+    code = KINDS.get(kind)
+    if code is None:
+        raise RuntimeError(f"{what}: kind must be one of {sorted(KINDS)}, got {kind!r}")
     n_pages, heads, blocks, rec = pool.shape
-    dev = pool.device
+    if rec % 32 != 16:
+        raise RuntimeError(f"{what}: the pool's records have {rec} bytes, not 32 * D + 16")
     if table.dim() != 2:
         raise RuntimeError(f"{what}: table must be [slots, columns]")
     n_slots, n_cols = table.shape
-    if indptr is not None:
-        if indptr.dim() != 1:
-            raise RuntimeError(f"{what}: indptr must be [sequences + 1]")
-        B = indptr.numel() - 1
-    else:
-        B = n_slots if slots is None else slots.numel()
-    head = (pool.data_ptr(), _kind(what, kind), n_pages, heads, (rec - 16) // 32,
-            blocks * BLOCK_TOKENS, _int32(what, "table", table, dev), n_slots, n_cols,
-            _int32(what, "lengths", lengths, dev, (n_slots,)),
-            _int32(what, "slots", slots, dev, (B,)))
-    if rec % 32 != 16:
-        raise RuntimeError(f"{what}: the pool's records have {rec} bytes, not 32 * D + 16")
-    return head, _int32(what, "indptr", indptr, dev), B
+    B = (indptr.numel() - 1 if indptr is not None else n_slots if slots is None
+         else slots.numel())
+    dim = rec // 32
+    return (pool.data_ptr(), code, n_pages, heads, dim, blocks * BLOCK_TOKENS,
+            _int32(what, "table", table, dev), n_slots, n_cols,
+            _int32(what, "lengths", lengths, dev, n_slots),
+            _int32(what, "slots", slots, dev, B)), \
+        _int32(what, "indptr", indptr, dev), B, heads, dim, dev
 
 
-def _rows(what: str, name: str, t, heads, dim, device):
-    """t [N, heads, dim] with 16-byte rows; copied when its strides do not allow that."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or t.device != device:
-        raise RuntimeError(f"{what}: {name} must be [rows, {heads}, {dim}] on {device}, "
+def _rows(what: str, name: str, t, heads, dim, dev: int):
+    """t [N, heads, dim] with 16-byte rows, and its strides; copied when they do not allow
+    that."""
+    if t.dim() != 3 or t.get_device() != dev or t.shape[1:] != (heads, dim):
+        raise RuntimeError(f"{what}: {name} must be [rows, {heads}, {dim}] on cuda:{dev}, "
                            f"got {tuple(t.shape)} on {t.device}")
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+    row, head, one = t.stride()
+    if one != 1 or row % 8 or head % 8 or t.data_ptr() % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-    return t
+        row, head, _ = t.stride()
+    return t, row, head
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, table: torch.Tensor,
@@ -125,16 +127,16 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, table: to
     and neither counts towards the scale. max_new is accepted for symmetry with
     paged_attention and not needed.
     """
-    head, ip, B = _cache_args("paged_append", pool, kind, table, lengths, slots, indptr, None)
-    heads, dim, dev = head[3], head[4], pool.device
-    k = _rows("paged_append", "k", k, heads, dim, dev)
-    v = _rows("paged_append", "v", v, heads, dim, dev)
-    if k.shape != v.shape or k.dtype != v.dtype or _DTYPES.get(k.dtype, 2) == 2:
+    what = "paged_append"
+    cache, ip, B, heads, dim, dev = _cache_args(what, pool, kind, table, lengths, slots, indptr)
+    k, k_row, k_head = _rows(what, "k", k, heads, dim, dev)
+    v, v_row, v_head = _rows(what, "v", v, heads, dim, dev)
+    code = _DTYPES.get(k.dtype, 2)
+    if k.shape != v.shape or k.dtype is not v.dtype or code == 2:
         raise RuntimeError("paged_append: k and v must have one shape and be fp16 or bf16")
     lib = get_cuda_ops().lib
-    _launch(lib.kvq_paged_append, lib, dev, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                                    v.stride(0), v.stride(1), _DTYPES[k.dtype], *head, ip, B,
-                                    k.shape[0])
+    _launch(lib.kvq_paged_append, lib, dev, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row,
+            v_head, code, *cache, ip, B, k.shape[0])
 
 
 def paged_read(pool: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, kind: str,
@@ -142,15 +144,15 @@ def paged_read(pool: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, k
                slots: torch.Tensor | None = None, dtype: torch.dtype = torch.float16):
     """The values (code * scale) of the tokens [starts[b], starts[b] + rows of b) of each
     sequence: (k, v), both [total, heads, D] in fp16, bf16 or fp32. starts None: from 0."""
-    head, ip, B = _cache_args("paged_read", pool, kind, table, lengths, slots, indptr, total)
-    if dtype not in _DTYPES:
+    what = "paged_read"
+    cache, ip, B, heads, dim, dev = _cache_args(what, pool, kind, table, lengths, slots, indptr)
+    code = _DTYPES.get(dtype)
+    if code is None:
         raise RuntimeError(f"paged_read: dtype must be fp16, bf16 or fp32, got {dtype}")
-    dev = pool.device
-    k = torch.empty((int(total), head[3], head[4]), dtype=dtype, device=dev)
-    v = torch.empty_like(k)
+    k, v = torch.empty((2, int(total), heads, dim), dtype=dtype, device=pool.device).unbind(0)
     lib = get_cuda_ops().lib
-    _launch(lib.kvq_paged_read, lib, dev, *head, _int32("paged_read", "starts", starts, dev, (B,)),
-                                  ip, B, int(total), k.data_ptr(), v.data_ptr(), _DTYPES[dtype])
+    _launch(lib.kvq_paged_read, lib, dev, *cache, _int32(what, "starts", starts, dev, B), ip, B,
+            int(total), k.data_ptr(), v.data_ptr(), code)
     return k, v
 
 
@@ -171,31 +173,31 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor,
     max_new: the most rows of any sequence (default: N when indptr is given; a smaller
     bound gives a better split); scale defaults to 1 / sqrt(D).
     """
-    head, ip, B = _cache_args("paged_attention", pool, kind, table, lengths, slots, indptr, None)
-    heads, dim, dev = head[3], head[4], pool.device
+    what = "paged_attention"
+    cache, ip, B, heads, dim, dev = _cache_args(what, pool, kind, table, lengths, slots, indptr)
     if q.dim() != 3 or q.shape[1] == 0 or q.shape[1] % heads:
         raise RuntimeError(f"paged_attention: q {tuple(q.shape)} does not match {heads} KV heads")
     N, Hq, _ = q.shape
-    q = _rows("paged_attention", "q", q, Hq, dim, dev)
-    if _DTYPES.get(q.dtype, 2) == 2:
+    q, row, head = _rows(what, "q", q, Hq, dim, dev)
+    code = _DTYPES.get(q.dtype, 2)
+    if code == 2:
         raise RuntimeError("paged_attention: q must be fp16 or bf16")
     if out is None:
-        out = torch.empty((N, Hq, dim), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev \
-            or not out.is_contiguous():
+        out = torch.empty((N, Hq, dim), dtype=q.dtype, device=q.device)
+    elif (out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != dev
+          or not out.is_contiguous()):
         raise RuntimeError("paged_attention: out must be contiguous, of q's shape and type")
-    if ml_out is not None and (ml_out.dtype != torch.float32 or not ml_out.is_contiguous()
-                               or ml_out.numel() != N * Hq * 2 or ml_out.device != dev):
+    if ml_out is not None and (ml_out.dtype is not torch.float32 or not ml_out.is_contiguous()
+                               or ml_out.numel() != N * Hq * 2 or ml_out.get_device() != dev):
         raise RuntimeError("paged_attention: ml_out must be contiguous fp32 [N, Hq, 2]")
     if max_new is None:
         max_new = N if indptr is not None else N // max(1, B)
     lib = get_cuda_ops().lib
-    need = lib.kvq_paged_attention_workspace(dim, int(max_new), Hq // heads)
-    ws = (workspace or DecodeWorkspace()).get(need, dev)
-    _launch(lib.kvq_paged_attention, lib, dev, 
-            q.data_ptr(), q.stride(0), q.stride(1), _DTYPES[q.dtype], Hq // heads, *head, ip, B, N,
-            int(max_new), 1.0 / math.sqrt(dim) if scale is None else float(scale), int(window),
-            out.data_ptr(), _ptr(ml_out), ws.data_ptr(), ws.numel())
+    need = lib.kvq_paged_attention_workspace(dim, max_new, Hq // heads)
+    ws = (workspace or DecodeWorkspace()).get(need, pool.device)
+    _launch(lib.kvq_paged_attention, lib, dev, q.data_ptr(), row, head, code, Hq // heads, *cache,
+            ip, B, N, max_new, dim ** -0.5 if scale is None else scale, window, out.data_ptr(),
+            _ptr(ml_out), ws.data_ptr(), ws.numel())
     return out
 
 
@@ -206,47 +208,49 @@ NO_PAGES, BAD_SLOT = 1, 2  # bits of `status`
 
 
 def _meta_args(what: str, table, lengths, refs, page_tokens):
-    if not table.is_cuda or table.dim() != 2:
+    dev = table.get_device()
+    if dev < 0 or table.dim() != 2:
         raise RuntimeError(f"{what}: table must be a CUDA tensor [slots, columns]")
-    dev = table.device
-    return (_int32(what, "table", table, dev), table.shape[0], table.shape[1],
-            _int32(what, "lengths", lengths, dev, (table.shape[0],)),
-            _int32(what, "refs", refs, dev), refs.numel(), int(page_tokens))
+    n_slots, n_cols = table.shape
+    return (_int32(what, "table", table, dev), n_slots, n_cols,
+            _int32(what, "lengths", lengths, dev, n_slots), _int32(what, "refs", refs, dev),
+            refs.numel(), page_tokens), dev
 
 
 def _pool_args(what: str, pool):
-    """(pointer, layers, bytes between layers, bytes of a page) of a pool [pages, ...] or
-    [layers, pages, ...]."""
-    if not pool.is_cuda or pool.dtype != torch.uint8 or pool.dim() not in (4, 5):
+    """(pointer, layers, bytes between layers, bytes of a page), pages and page tokens of a
+    pool [pages, ...] or [layers, pages, ...]."""
+    if not pool.is_cuda or pool.dtype is not torch.uint8 or pool.dim() not in (4, 5):
         raise RuntimeError(f"{what}: pool must be a CUDA uint8 tensor [pages, heads, blocks, "
                            "record] or [layers, pages, heads, blocks, record]")
     if not pool.is_contiguous():
         raise RuntimeError(f"{what}: pool must be contiguous")
-    page = pool.shape[-3] * pool.shape[-2] * pool.shape[-1]
-    layers = pool.shape[0] if pool.dim() == 5 else 1
-    return pool.data_ptr(), layers, pool.shape[-4] * page, page
+    *layers, pages, heads, blocks, rec = pool.shape
+    page = heads * blocks * rec
+    return (pool.data_ptr(), layers[0] if layers else 1, pages * page, page), pages, \
+        blocks * BLOCK_TOKENS
 
 
 def paged_free(table, lengths, refs, slots, page_tokens: int, status) -> None:
     """Gives up the pages of the slots (int32): counts down, rows -1, lengths 0. status
     (int32 [1]) gets BAD_SLOT for a slot out of range or named twice, which is skipped."""
-    meta = _meta_args("paged_free", table, lengths, refs, page_tokens)
-    dev = table.device
+    what = "paged_free"
+    meta, dev = _meta_args(what, table, lengths, refs, page_tokens)
     lib = get_cuda_ops().lib
-    _launch(lib.kvq_paged_free, lib, dev, *meta, _int32("paged_free", "slots", slots, dev), slots.numel(),
-                                  _int32("paged_free", "status", status, dev, (1,)))
+    _launch(lib.kvq_paged_free, lib, dev, *meta, _int32(what, "slots", slots, dev), slots.numel(),
+            _int32(what, "status", status, dev, 1))
 
 
 def paged_fork(table, lengths, refs, src, dst, page_tokens: int, status) -> None:
     """dst[i] becomes a copy of src[i] that shares all its pages (an open last page too:
     paged_extend gives a writer its own copy). A pair whose dst holds tokens, is a src,
     is named twice or is out of range is skipped and sets BAD_SLOT in status."""
-    meta = _meta_args("paged_fork", table, lengths, refs, page_tokens)
-    dev = table.device
+    what = "paged_fork"
+    meta, dev = _meta_args(what, table, lengths, refs, page_tokens)
+    n = src.numel()
     lib = get_cuda_ops().lib
-    _launch(lib.kvq_paged_fork, lib, dev, *meta, _int32("paged_fork", "src", src, dev),
-                                  _int32("paged_fork", "dst", dst, dev, tuple(src.shape)),
-                                  src.numel(), _int32("paged_fork", "status", status, dev, (1,)))
+    _launch(lib.kvq_paged_fork, lib, dev, *meta, _int32(what, "src", src, dev),
+            _int32(what, "dst", dst, dev, n), n, _int32(what, "status", status, dev, 1))
 
 
 def paged_extend(pool, table, lengths, refs, slots, n_new, status,
@@ -260,19 +264,17 @@ def paged_extend(pool, table, lengths, refs, slots, n_new, status,
     (BAD_SLOT), nothing changes.
     """
     what = "paged_extend"
-    ptr, layers, stride, page = _pool_args(what, pool)
-    meta = _meta_args(what, table, lengths, refs, pool.shape[-2] * BLOCK_TOKENS)
-    dev = table.device
-    if refs.numel() != pool.shape[-4] or pool.device != dev:
+    where, pages, page_tokens = _pool_args(what, pool)
+    meta, dev = _meta_args(what, table, lengths, refs, page_tokens)
+    if meta[5] != pages or pool.get_device() != dev:
         raise RuntimeError(f"{what}: refs must have one entry per page of the pool")
+    n = slots.numel()
     each = isinstance(n_new, torch.Tensor)
     lib = get_cuda_ops().lib
-    ws = (workspace or DecodeWorkspace()).get(lib.kvq_paged_extend_workspace(refs.numel()), dev)
-    _launch(lib.kvq_paged_extend, lib, dev, 
-            ptr, layers, stride, page, *meta, _int32(what, "slots", slots, dev), slots.numel(),
-            _int32(what, "n_new", n_new, dev, tuple(slots.shape)) if each else None,
-            0 if each else int(n_new), _int32(what, "status", status, dev, (1,)), ws.data_ptr(),
-            ws.numel())
+    ws = (workspace or DecodeWorkspace()).get(lib.kvq_paged_extend_workspace(pages), pool.device)
+    _launch(lib.kvq_paged_extend, lib, dev, *where, *meta, _int32(what, "slots", slots, dev), n,
+            _int32(what, "n_new", n_new, dev, n) if each else None, 0 if each else n_new,
+            _int32(what, "status", status, dev, 1), ws.data_ptr(), ws.numel())
 
 
 def paged_compact(pool, table, refs, workspace: DecodeWorkspace | None = None,
@@ -281,18 +283,17 @@ def paged_compact(pool, table, refs, workspace: DecodeWorkspace | None = None,
     ascending order, into the free ones below it, in every layer; table and refs follow.
     Returns the number of live pages (int32 [1] on the device)."""
     what = "paged_compact"
-    ptr, layers, stride, page = _pool_args(what, pool)
-    dev = table.device
-    if refs.numel() != pool.shape[-4] or pool.device != dev or table.dim() != 2:
+    where, pages, _ = _pool_args(what, pool)
+    dev = table.get_device()
+    if refs.numel() != pages or pool.get_device() != dev or table.dim() != 2:
         raise RuntimeError(f"{what}: refs must have one entry per page of the pool")
     if n_live is None:
-        n_live = torch.empty(1, dtype=torch.int32, device=dev)
+        n_live = torch.empty(1, dtype=torch.int32, device=pool.device)
     lib = get_cuda_ops().lib
-    ws = (workspace or DecodeWorkspace()).get(lib.kvq_paged_extend_workspace(refs.numel()), dev)
-    _launch(lib.kvq_paged_compact, lib, dev, 
-            ptr, layers, stride, page, _int32(what, "table", table, dev), table.shape[0],
-            table.shape[1], _int32(what, "refs", refs, dev), refs.numel(),
-            _int32(what, "n_live", n_live, dev, (1,)), ws.data_ptr(), ws.numel())
+    ws = (workspace or DecodeWorkspace()).get(lib.kvq_paged_extend_workspace(pages), pool.device)
+    _launch(lib.kvq_paged_compact, lib, dev, *where, _int32(what, "table", table, dev),
+            *table.shape, _int32(what, "refs", refs, dev), pages,
+            _int32(what, "n_live", n_live, dev, 1), ws.data_ptr(), ws.numel())
     return n_live
 
 
@@ -300,15 +301,14 @@ def paged_copy(src_pool, dst_pool, src, dst, workspace: DecodeWorkspace | None =
     """Copies pages src[i] of src_pool to pages dst[i] of dst_pool (which may be the same
     pool), every layer. dst pages are distinct, and in one pool none of them is in src."""
     what = "paged_copy"
-    sp, layers, s_stride, page = _pool_args(what, src_pool)
-    dp, d_layers, d_stride, d_page = _pool_args(what, dst_pool)
-    dev = src_pool.device
-    if layers != d_layers or page != d_page or dst_pool.device != dev:
+    (sp, layers, s_stride, page), s_pages, _ = _pool_args(what, src_pool)
+    (dp, d_layers, d_stride, d_page), d_pages, _ = _pool_args(what, dst_pool)
+    dev = src_pool.get_device()
+    if layers != d_layers or page != d_page or dst_pool.get_device() != dev:
         raise RuntimeError(f"{what}: the pools differ in layers, page size or device")
     n = src.numel()
     lib = get_cuda_ops().lib
-    ws = (workspace or DecodeWorkspace()).get(lib.kvq_paged_copy_workspace(n), dev)
-    _launch(lib.kvq_paged_copy, lib, dev, 
-            sp, src_pool.shape[-4], s_stride, dp, dst_pool.shape[-4], d_stride, layers, page,
-            _int32(what, "src", src, dev), _int32(what, "dst", dst, dev, tuple(src.shape)), n,
+    ws = (workspace or DecodeWorkspace()).get(lib.kvq_paged_copy_workspace(n), src_pool.device)
+    _launch(lib.kvq_paged_copy, lib, dev, sp, s_pages, s_stride, dp, d_pages, d_stride, layers,
+            page, _int32(what, "src", src, dev), _int32(what, "dst", dst, dev, n), n,
             ws.data_ptr(), ws.numel())
