@@ -633,6 +633,75 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
   }
 }
 
+// A warp's part of joining the n pieces of a row: pieces part, part + split, ..,
+// weighted by 2^(their reference - the largest of all). piece(i) gives the place of
+// piece i, its rows first, then (reference, sum, maximum, -) of each. The lane's
+// channels are C * lane .. + C - 1; l is the lane's share of the sum.
+template <int D, typename Piece>
+__device__ __forceinline__ void join_row(int n, int part, int split, int rows, int r, Piece piece,
+                                         int lane, float (&o)[D / 32], float& m, float& m2,
+                                         float& l) {
+  constexpr int C = D / 32;
+  m = m2 = -INFINITY;
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < C; ++i) o[i] = 0.f;
+  float4 own = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);  // of piece part + split * lane
+  if (part + split * lane < n)
+    own = *reinterpret_cast<const float4*>(piece(part + split * lane) + rows * D + 4 * r);
+  m2 = own.x;
+  m = own.z;
+  if (split > 1 || n > 32) {
+    for (int i = lane; i < n; i += 32) {
+      const float4 q = *reinterpret_cast<const float4*>(piece(i) + rows * D + 4 * r);
+      m2 = fmaxf(m2, q.x);
+      m = fmaxf(m, q.z);
+    }
+  }
+  m2 = warp_max(m2);
+  m = warp_max(m);
+  const float ref = m2 == -INFINITY ? 0.f : m2;
+  for (int i0 = part; i0 < n; i0 += 32 * split) {  // pieces i0, i0 + split, ..
+    float f = 0.f;
+    const int mine = i0 + split * lane;
+    if (mine < n) {
+      const float4 q =
+          i0 == part ? own : *reinterpret_cast<const float4*>(piece(mine) + rows * D + 4 * r);
+      f = exp2_approx(q.x - ref);
+      l = fmaf(q.y, f, l);
+    }
+    const int k = min(32, (n - i0 + split - 1) / split);
+#pragma unroll 8
+    for (int i = 0; i < k; ++i) {
+      const float w = __shfl_sync(0xffffffffu, f, i);
+      const float* p = piece(i0 + split * i) + r * D + C * lane;
+      float x[C];
+      if constexpr (C == 4) {
+        const float4 y = *reinterpret_cast<const float4*>(p);
+        x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
+      } else {
+        const float2 y = *reinterpret_cast<const float2*>(p);
+        x[0] = y.x; x[1] = y.y;
+      }
+#pragma unroll
+      for (int e = 0; e < C; ++e) o[e] = fmaf(x[e], w, o[e]);
+    }
+  }
+}
+
+// A joined row's output and statistics (l: the whole sum).
+template <int D, typename T>
+__device__ __forceinline__ void store_row(const AttnArgs& a, int64_t at, int lane,
+                                          const float (&o)[D / 32], float m, float m2, float l) {
+  const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+  T* out = (T*)a.out + at * D + D / 32 * lane;
+#pragma unroll
+  for (int e = 0; e < D / 32; e += 2)
+    *reinterpret_cast<uint32_t*>(out + e) =
+        l == 0.f ? 0u : from_float2<T>(o[e] * inv, o[e + 1] * inv);
+  if (a.ml && lane == 0) a.ml[at] = row_stats(m, m2, l);
+}
+
 // Joins the pieces of the units that several workers share, in a fixed order. A
 // CTA takes `rows` of the unit_rows rows that a unit can have, 4 / rows warps each
 // (few units have many pieces); a lane adds D / 32 channels of its warp's pieces,
@@ -667,53 +736,12 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttnArgs a, i
   const int64_t w1 = here ? (x1 * W - 1) / total : 0;
   wait_previous();
   const int n = w1 > w0 ? (int)(w1 - w0) + 1 : 0;  // the row's pieces (0: nothing to join)
-  float m = -INFINITY, m2 = -INFINITY, l = 0.f, o[C];
-#pragma unroll
-  for (int i = 0; i < C; ++i) o[i] = 0.f;
-  auto piece = [&](int i) {  // the first piece is its worker's last, the others their first
-    return a.part + (2 * (w0 + i) + (i == 0)) * part_floats(D, NT);
-  };
-  float4 own = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);  // of piece part + split * lane
-  if (part + split * lane < n)
-    own = *reinterpret_cast<const float4*>(piece(part + split * lane) + R * D + 4 * r);
-  m2 = own.x;
-  m = own.z;
-  if (split > 1 || n > 32) {
-    for (int i = lane; i < n; i += 32) {
-      const float4 q = *reinterpret_cast<const float4*>(piece(i) + R * D + 4 * r);
-      m2 = fmaxf(m2, q.x);
-      m = fmaxf(m, q.z);
-    }
-  }
-  m2 = warp_max(m2);
-  m = warp_max(m);
-  const float ref = m2 == -INFINITY ? 0.f : m2;
-  for (int i0 = part; i0 < n; i0 += 32 * split) {  // pieces i0, i0 + split, ..
-    float f = 0.f;
-    const int mine = i0 + split * lane;
-    if (mine < n) {
-      const float4 q =
-          i0 == part ? own : *reinterpret_cast<const float4*>(piece(mine) + R * D + 4 * r);
-      f = exp2_approx(q.x - ref);
-      l = fmaf(q.y, f, l);
-    }
-    const int k = min(32, (n - i0 + split - 1) / split);
-#pragma unroll 8
-    for (int i = 0; i < k; ++i) {
-      const float w = __shfl_sync(0xffffffffu, f, i);
-      const float* p = piece(i0 + split * i) + r * D + C * lane;
-      float x[C];
-      if constexpr (C == 4) {
-        const float4 y = *reinterpret_cast<const float4*>(p);
-        x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
-      } else {
-        const float2 y = *reinterpret_cast<const float2*>(p);
-        x[0] = y.x; x[1] = y.y;
-      }
-#pragma unroll
-      for (int e = 0; e < C; ++e) o[e] = fmaf(x[e], w, o[e]);
-    }
-  }
+  float m, m2, l, o[C];
+  // the first piece is its worker's last, the others their workers' first
+  join_row<D>(
+      n, part, split, R, r,
+      [&](int i) { return a.part + (2 * (w0 + i) + (i == 0)) * part_floats(D, NT); }, lane, o, m,
+      m2, l);
   l = warp_sum(l);
   if (split > 1) {
 #pragma unroll
@@ -730,19 +758,17 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttnArgs a, i
   if (n == 0) return;
   const int64_t at = (s.r0 + row / a.group) * ((int64_t)a.v.heads * a.group) + h * a.group +
                      row % a.group;
-  const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
-  T* out = (T*)a.out + at * D + C * lane;
-#pragma unroll
-  for (int e = 0; e < C; e += 2)
-    *reinterpret_cast<uint32_t*>(out + e) =
-        l == 0.f ? 0u : from_float2<T>(o[e] * inv, o[e + 1] * inv);
-  if (a.ml && lane == 0) a.ml[at] = row_stats(m, m2, l);
+  store_row<D, T>(a, at, lane, o, m, m2, l);
 }
 
-// Rows of a call's largest sequence: 8-row tiles where one or two are enough,
-// else (0) the 128-row tiles of kvq_paged_tile.cuh.
+// Rows of a call's largest sequence: 8-row tiles where one is enough, up to three
+// groups of two, else (0) the 128-row tiles of kvq_paged_tile.cuh. 23 sequences of up
+// to 6000 tokens, window 2500, D = 64 / 128: 48 rows 84 / 107 us in groups against
+// 101 / 136 in tiles, 64 rows 108 / 137 against 102 / 140; one of 32768 tokens: 32
+// rows 51 against 62, 64 rows 77 against 65.
+constexpr int kGroupRows = 48;
 inline int row_tiles(int64_t max_new, int64_t group) {
-  return max_new * group <= 8 ? 1 : max_new * group <= 16 ? 2 : 0;
+  return max_new * group <= 8 ? 1 : max_new * group <= kGroupRows ? 2 : 0;
 }
 
 // Allows `kernel` `bytes` of dynamic shared memory on the current device; `done` is

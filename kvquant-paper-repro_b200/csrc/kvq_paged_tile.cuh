@@ -677,8 +677,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
 }
 
 // Joins a unit that the shares' ends cut: the CTA column of the unit's first
-// inner cut adds its pieces in order, 32 rows per CTA.
-constexpr int kTileJoinRows = 32, kTileJoinThreads = 256;
+// inner cut adds its pieces in order, 16 rows per CTA, two per warp.
+constexpr int kTileJoinRows = 16, kTileJoinThreads = 256;
 
 template <int D, typename T>
 __global__ void __launch_bounds__(kTileJoinThreads) tile_join_kernel(AttnArgs a) {
@@ -698,26 +698,23 @@ __global__ void __launch_bounds__(kTileJoinThreads) tile_join_kernel(AttnArgs a)
   c.next(a, pre, threadIdx.x & 31);
   const int64_t start = x - c.first, end = start + c.n_unit;
   if (c.first == 0 || total * (cut - 1) / W > start) return;
-  constexpr int G = kTileJoinThreads / D, F = kUnitRows * (D + 4);
-  const int d = threadIdx.x % D;
-  for (int i = threadIdx.x / D; i < kTileJoinRows; i += G) {
+  int n = 1;  // pieces: of the worker before the cut, and on to the unit's end
+  while (cut - 1 + n < W && total * (cut - 1 + n) / W < end) ++n;
+  const int lane = threadIdx.x & 31;
+  for (int i = threadIdx.x >> 5; i < kTileJoinRows; i += kTileJoinThreads / 32) {
     const int ur = blockIdx.y * kTileJoinRows + i, r = c.row0 + ur;
     if (r >= c.s.n * a.group) return;
-    float m = -INFINITY, ref = -INFINITY, l = 0.f, o = 0.f;
-    for (int64_t w = cut - 1; w < W && total * w / W < end; ++w) {
-      const float* p = a.part + (2 * w + (w == cut - 1)) * F;
-      const float4 q = *reinterpret_cast<const float4*>(p + kUnitRows * D + 4 * ur);
-      const float now = fmaxf(ref, q.x), base = now == -INFINITY ? 0.f : now;
-      const float f0 = exp2_approx(ref - base), f1 = exp2_approx(q.x - base);
-      o = o * f0 + p[ur * D + d] * f1;
-      l = l * f0 + q.y * f1;
-      m = fmaxf(m, q.z);
-      ref = now;
-    }
+    float m, ref, l, o[D / 32];
+    join_row<D>(
+        n, 0, 1, kUnitRows, ur,
+        [&](int j) {
+          return a.part + (2 * (cut - 1 + j) + (j == 0)) * (kUnitRows * (D + 4));
+        },
+        lane, o, m, ref, l);
+    l = warp_sum(l);
     const int64_t at = (c.s.r0 + r / a.group) * ((int64_t)a.v.heads * a.group) +
                        c.h * a.group + r % a.group;
-    ((T*)a.out)[at * D + d] = from_float<T>(l == 0.f ? 0.f : o * __fdiv_rn(1.f, l));
-    if (a.ml && d == 0) a.ml[at] = row_stats(m, ref, l);
+    store_row<D, T>(a, at, lane, o, m, ref, l);
   }
 }
 
@@ -730,8 +727,11 @@ static int launch_attend_tile(AttnArgs a, cudaStream_t st) {
   int rc = launch_next("paged_attention (tiles)", attend_tile_kernel<D, KIND, T>, dim3(kSms),
                        kTileThreads, smem, st, a);
   if (rc) return rc;
+  const int64_t rows = (int64_t)a.max_new * a.group;
+  const int unit_rows = rows < kUnitRows ? (int)rows : kUnitRows;
   return launch_next("paged_attention (tile join)", tile_join_kernel<D, T>,
-                     dim3(kSms - 1, kUnitRows / kTileJoinRows), kTileJoinThreads,
+                     dim3(kSms - 1, (unit_rows + kTileJoinRows - 1) / kTileJoinRows),
+                     kTileJoinThreads,
                      (int)((a.v.B + 1) * sizeof(int32_t)), st, a);
 }
 
