@@ -466,13 +466,17 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
     }
     bool more = c.next(a, R, sm.pre, cache);
     uint32_t k = 0;  // records issued
-    int i = 0, col = 0, in_page = 0;
+    int i = 0, col = 0, in_page = 0, ahead = -1;
     const uint8_t *page = nullptr, *rec = nullptr;
-    // The next record's address is ready before its place is: the table is read
-    // while the lane polls.
-    auto find_page = [&]() {
-      const int p = col * a.v.blocks * kBlock < c.s.len
-                        ? a.v.table[(int64_t)c.s.slot * a.v.n_cols + col] : -1;
+    // The next record's address is ready before its place is, and the table is read
+    // a page ahead, so that a lane that polls waits for no memory.
+    auto page_id = [&](int at) {
+      return at * a.v.blocks * kBlock < c.s.len ? a.v.table[(int64_t)c.s.slot * a.v.n_cols + at]
+                                                : -1;
+    };
+    auto take_page = [&]() {
+      const int p = ahead;
+      ahead = page_id(col + 1);
       if (p >= 0 && p < a.v.n_pages) {
         page = a.v.pool + p * a.v.page_bytes() + c.unit / c.s.groups * a.v.head_bytes();
       } else {
@@ -485,16 +489,18 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
         const int blk = c.s.lo_blk + c.blk0;
         col = blk / a.v.blocks;
         in_page = blk % a.v.blocks;
-        find_page();
+        ahead = page_id(col);
+        take_page();
       } else if (++in_page == a.v.blocks) {
         in_page = 0;
         ++col;
-        find_page();
+        take_page();
       }
       rec = page ? page + (int64_t)in_page * rec_bytes(D) : nullptr;
     };
     if (more) find_record();
-    unsigned long long t0 = sm100::global_ns();
+    uint32_t polls = 0;
+    unsigned long long t0 = 0;
     while (__any_sync(0xffffffffu, more)) {
       if (more) {
         const int st = k % S;
@@ -512,11 +518,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
             more = c.next(a, R, sm.pre, cache);
           }
           if (more) find_record();
-          t0 = sm100::global_ns();
-        } else if (*abort || sm100::global_ns() - t0 > sm100::kWaitLimitNs) {
-          *abort = 1;
-          atomicOr(&g_status, 2);
-          more = false;
+          polls = 0;
+        } else if ((++polls & 255) == 0) {  // the clock is slow to read
+          if (polls == 256) t0 = sm100::global_ns();
+          if (*abort || sm100::global_ns() - t0 > sm100::kWaitLimitNs) {
+            *abort = 1;
+            atomicOr(&g_status, 2);
+            more = false;
+          }
         }
       }
       __syncwarp();
