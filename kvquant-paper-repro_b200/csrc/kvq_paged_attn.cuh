@@ -375,8 +375,11 @@ __device__ __forceinline__ void let_next_start() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-constexpr int kAttnWarps = 8;  // consumers; one more warp feeds them
-constexpr int kAttnThreads = 32 * (kAttnWarps + 1);
+// 8 consumer warps, and 4 that feed two each. A copy is issued for one lane at a time
+// (~190 cycles each), so one warp that fed all eight was what bound the kernel: 1500
+// cycles for 8 records, the rate of HBM itself (16 x 5 rows, window 2500: 55 us).
+constexpr int kAttnWarps = 8, kFeeds = 2;
+constexpr int kAttnThreads = 32 * (kAttnWarps + kAttnWarps / kFeeds);
 constexpr int kSms = 148;
 
 template <int D>
@@ -429,9 +432,9 @@ struct Cursor {
 };
 
 // One CTA per SM. Every consumer warp works through its own share of the blocks
-// with its own ring of records, so no warp waits for another one; a lane of the
-// ninth warp keeps each ring full: one bulk copy per record, ring after ring
-// across the ends of units. 8 warps hide the ~500 cycles a block takes a warp
+// with its own ring of records, so no warp waits for another one; a lane of a
+// feeding warp keeps each ring full: one bulk copy per record, on across the ends of
+// units. 8 warps hide the ~500 cycles a block takes a warp
 // (HBM delivers one per ~180 cycles and SM).
 template <int D, int KIND, int NT, typename T>
 __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
@@ -455,12 +458,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
   const int64_t W = workers_of(a, total);
   volatile int* abort = &sm.abort;
 
-  if (warp == kAttnWarps) {
-    // lane w feeds warp w; lanes poll, none waits for another one's ring
-    const int64_t w = (int64_t)lane * gridDim.x + blockIdx.x;
+  if (warp >= kAttnWarps) {
+    // a lane feeds warp `to`; lanes poll, none waits for another one's ring
+    const int to = (warp - kAttnWarps) * kFeeds + lane % kFeeds;
+    const int64_t w = (int64_t)to * gridDim.x + blockIdx.x;
     Cursor c;
     c.x = c.end = 0;
-    if (lane < kAttnWarps && w < W) {
+    if (lane < kFeeds && w < W) {
       c.x = total * w / W;
       c.end = total * (w + 1) / W;
     }
@@ -504,13 +508,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
     while (__any_sync(0xffffffffu, more)) {
       if (more) {
         const int st = k % S;
-        if (k < S || sm100::mbar_poll(&sm.empty[lane][st], (k / S - 1) & 1)) {
-          sm.skip[lane][st] = rec == nullptr;
+        if (k < S || sm100::mbar_poll(&sm.empty[to][st], (k / S - 1) & 1)) {
+          sm.skip[to][st] = rec == nullptr;
           if (rec) {
-            sm100::mbar_arrive_expect_tx(&sm.full[lane][st], rec_bytes(D));
-            sm100::bulk_g2s(sm.ring[lane][st], rec, rec_bytes(D), &sm.full[lane][st]);
+            sm100::mbar_arrive_expect_tx(&sm.full[to][st], rec_bytes(D));
+            sm100::bulk_g2s(sm.ring[to][st], rec, rec_bytes(D), &sm.full[to][st]);
           } else {
-            sm100::mbar_arrive(&sm.full[lane][st]);
+            sm100::mbar_arrive(&sm.full[to][st]);
           }
           ++k;
           if (++i == c.n) {
@@ -535,7 +539,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
       const uint32_t q = k - 1 - j;
       if (k == 0 || (uint32_t)j >= k) break;
       t0 = sm100::global_ns();
-      while (!sm100::mbar_test(&sm.full[lane][q % S], (q / S) & 1) &&
+      while (!sm100::mbar_test(&sm.full[to][q % S], (q / S) & 1) &&
              sm100::global_ns() - t0 < sm100::kWaitLimitNs) {
       }
     }
