@@ -659,12 +659,29 @@ __device__ __forceinline__ void join_row(int n, int part, int split, int rows, i
   l = 0.f;
 #pragma unroll
   for (int i = 0; i < C; ++i) o[i] = 0.f;
+  auto load = [&](int i, float (&x)[C]) {
+    const float* p = piece(i) + r * D + C * lane;
+    if constexpr (C == 4) {
+      const float4 y = *reinterpret_cast<const float4*>(p);
+      x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
+    } else {
+      const float2 y = *reinterpret_cast<const float2*>(p);
+      x[0] = y.x; x[1] = y.y;
+    }
+  };
+  // the first pieces and all statistics are fetched together
+  constexpr int kAhead = 4;
+  float first[kAhead][C];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (part + split * i < n) load(part + split * i, first[i]);
   float4 own = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);  // of piece part + split * lane
   if (part + split * lane < n)
     own = *reinterpret_cast<const float4*>(piece(part + split * lane) + rows * D + 4 * r);
   m2 = own.x;
   m = own.z;
   if (split > 1 || n > 32) {
+#pragma unroll 4
     for (int i = lane; i < n; i += 32) {
       const float4 q = *reinterpret_cast<const float4*>(piece(i) + rows * D + 4 * r);
       m2 = fmaxf(m2, q.x);
@@ -684,18 +701,21 @@ __device__ __forceinline__ void join_row(int n, int part, int split, int rows, i
       l = fmaf(q.y, f, l);
     }
     const int k = min(32, (n - i0 + split - 1) / split);
-#pragma unroll 8
-    for (int i = 0; i < k; ++i) {
-      const float w = __shfl_sync(0xffffffffu, f, i);
-      const float* p = piece(i0 + split * i) + r * D + C * lane;
-      float x[C];
-      if constexpr (C == 4) {
-        const float4 y = *reinterpret_cast<const float4*>(p);
-        x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
-      } else {
-        const float2 y = *reinterpret_cast<const float2*>(p);
-        x[0] = y.x; x[1] = y.y;
+    int i = 0;
+    if (i0 == part) {
+#pragma unroll
+      for (; i < kAhead; ++i) {
+        const float w = __shfl_sync(0xffffffffu, f, i);
+        if (i < k)
+#pragma unroll
+          for (int e = 0; e < C; ++e) o[e] = fmaf(first[i][e], w, o[e]);
       }
+    }
+#pragma unroll 8
+    for (; i < k; ++i) {
+      const float w = __shfl_sync(0xffffffffu, f, i);
+      float x[C];
+      load(i0 + split * i, x);
 #pragma unroll
       for (int e = 0; e < C; ++e) o[e] = fmaf(x[e], w, o[e]);
     }
