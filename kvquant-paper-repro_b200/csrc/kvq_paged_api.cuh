@@ -8,9 +8,9 @@ namespace paged {
 
 inline size_t attention_bytes(int64_t D, int64_t max_new, int64_t group) {
   const int NT = row_tiles(max_new, group);
-  const size_t floats = NT ? (size_t)kAttnWarps * part_floats((int)D, NT)
-                           : (size_t)kUnitRows * (D + 4);
-  return 2 * kSms * floats * sizeof(float);
+  if (NT == 0)
+    return kTileParts * kUnitRows * (D + 4) * sizeof(float) + (kMaxSeqs + 1) * sizeof(int32_t);
+  return (size_t)2 * kSms * kAttnWarps * part_floats((int)D, NT) * sizeof(float);
 }
 
 }  // namespace paged

@@ -23,13 +23,15 @@ namespace paged {
 
 constexpr int kTileRows = 128, kUnitRows = 256, kTileTok = 128;
 constexpr int kTileRecs = kTileTok / kBlock;  // records of a token tile
-constexpr int kRawStages = 12, kSlots = 3;
+constexpr int kGroupRecs = 4, kGroups = 4;  // records come in groups of 64 tokens
+constexpr int kRawStages = kGroups * kGroupRecs, kSlots = 3;
 constexpr int kTileThreads = 16 * 32;  // warps 14 and 15 only complete their warpgroup
 // Registers per thread of the warpgroups (softmax twice, dequantising, products and
 // copies): together the 4 x 128 of the launch. The softmax keeps a row's 128 scores.
 constexpr int kRegsSoftmax = 192, kRegsDequant = 80, kRegsIssue = 48;
 static_assert(2 * kRegsSoftmax + kRegsDequant + kRegsIssue <= 4 * 128, "register shares");
 constexpr int kDequantWarp = 8, kMmaWarp = 12, kLoadWarp = 13;
+constexpr int64_t kTileParts = 2 * kSms;  // pieces in the workspace, then B + 1 int32
 constexpr float kLazy = 8.f;  // the maximum may grow by 2^8 before O is rescaled
 
 template <int D>
@@ -37,7 +39,7 @@ struct TileSmem {
   alignas(128) uint8_t q[2][kTileRows * D * 2];
   alignas(128) uint8_t slot[kSlots][kTileTok * D * 2];  // K and V tiles in turn
   alignas(128) uint8_t raw[kRawStages][rec_bytes(D)];
-  uint64_t raw_full[kRawStages], raw_empty[kRawStages];
+  uint64_t raw_full[kGroups], raw_empty[kGroups];
   uint64_t slot_full[kSlots], slot_empty[kSlots];
   uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain;
   float4 scale[2][kTileRecs];  // (key scale, log2 value scale, 1 / value scale, -) of a tile
@@ -45,7 +47,6 @@ struct TileSmem {
   int skip[kRawStages];
   uint32_t tmem;
   int abort;
-  int32_t pre[1];  // B + 1
 };
 
 // Token tiles [t0, t0 + n) that row group r of a sequence sees (at least one).
@@ -58,7 +59,8 @@ __device__ __forceinline__ void unit_tiles(const AttnArgs& a, const Seq& s, int 
   n = max(1, max(p1, 0) / kTileTok - t0 + 1);
 }
 
-// As block_prefix, over token tiles.
+// As block_prefix, over token tiles; pre may be in global memory, where every CTA
+// writes the same values and reads its own.
 template <int THREADS>
 __device__ __forceinline__ int64_t tile_prefix(const AttnArgs& a, int32_t* pre, int64_t* sums) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
@@ -351,9 +353,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   volatile int* abort = &sm.abort;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kRawStages; ++i) {
+    for (int i = 0; i < kGroups; ++i) {
       mbar_init(&sm.raw_full[i], 1);
-      mbar_init(&sm.raw_empty[i], 1);
+      mbar_init(&sm.raw_empty[i], kGroupRecs);
     }
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&sm.slot_full[i], 4);
@@ -371,7 +373,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
   }
   wait_previous();
   let_next_start();  // only now: the join reads lengths before its own wait
-  const int64_t total = tile_prefix<kTileThreads>(a, sm.pre, sm.sums);  // syncs the block
+  int32_t* pre = reinterpret_cast<int32_t*>(a.part + kTileParts * kUnitRows * (D + 4));
+  const int64_t total = tile_prefix<kTileThreads>(a, pre, sm.sums);  // syncs the block
   const int64_t W = tile_workers(total);
   if (total == 0 || blockIdx.x >= W) return;
   if (warp == kMmaWarp) tmem_alloc(&sm.tmem, 512);
@@ -384,66 +387,54 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
   c.end = total * (blockIdx.x + 1) / W;
   uint32_t gi = 0;  // token tiles before the current one
 
+  // A lane is issued one copy at a time (~190 cycles), so records that lie one after
+  // another in a page come in one copy: a group is one to four copies.
   auto load_role = [&]() {
-    uint32_t issued = 0;
-    const int j = lane;
+    uint32_t groups = 0;
     bool ok = true;
-    while (ok && c.next(a, sm.pre, lane)) {
-      for (int i = 0; ok && i < c.n; ++i, ++gi) {
-        const uint32_t k = gi * kTileRecs + j, st = k % kRawStages, use = k / kRawStages;
-        if (j < kTileRecs) {
-          const unsigned long long t0 = global_ns();
-          while (use > 0 && !mbar_test(&sm.raw_empty[st], (use - 1) & 1)) {
-            if (*abort || global_ns() - t0 > kWaitLimitNs) {
-              *abort = 1;
-              atomicOr(&g_status, 2);
-              ok = false;
-              break;
-            }
-          }
-          if (ok) {
-            const int blk = (c.t0 + c.first + i) * kTileRecs + j;
-            const uint8_t* rec =
-                blk * kBlock < c.s.len ? a.v.record(c.s.slot, blk, c.h) : nullptr;
-            sm.skip[st] = rec == nullptr;
-            if (rec) {
-              mbar_arrive_expect_tx(&sm.raw_full[st], rec_bytes(D));
-              bulk_g2s(sm.raw[st], rec, rec_bytes(D), &sm.raw_full[st]);
-            } else {
-              mbar_arrive(&sm.raw_full[st]);
-            }
-            issued = k + 1;
-          }
+    while (ok && c.next(a, pre, lane)) {
+      for (int i = 0; ok && i < 2 * c.n; ++i, ++groups) {
+        const uint32_t st = groups % kGroups, use = groups / kGroups;
+        if (use > 0 && !mbar_wait(&sm.raw_empty[st], (use - 1) & 1, abort)) {
+          ok = false;
+          break;
         }
-        ok = __all_sync(0xffffffffu, ok);
+        const int blk = (c.t0 + c.first) * kTileRecs + i * kGroupRecs + lane;
+        const uint8_t* rec = lane < kGroupRecs && blk * kBlock < c.s.len
+                                 ? a.v.record(c.s.slot, blk, c.h) : nullptr;
+        const uint32_t have = __ballot_sync(0xffffffffu, rec != nullptr);
+        if (lane < kGroupRecs) sm.skip[st * kGroupRecs + lane] = rec == nullptr;
+        __syncwarp();
+        if (lane == 0) {
+          if (have) mbar_arrive_expect_tx(&sm.raw_full[st], __popc(have) * rec_bytes(D));
+          else mbar_arrive(&sm.raw_full[st]);
+        }
+        __syncwarp();
+        // the lane of a page's first record in the group copies all of them
+        if (rec && (lane == 0 || blk % a.v.blocks == 0)) {
+          int n = min(kGroupRecs - lane, a.v.blocks - blk % a.v.blocks);
+          n = min(n, __ffs(~(have >> lane)) - 1);
+          bulk_g2s(sm.raw[st * kGroupRecs + lane], rec, n * rec_bytes(D), &sm.raw_full[st]);
+        }
+        __syncwarp();
       }
     }
-    // the copies in flight land before the block ends: each stage's last record,
-    // i.e. those that no later one (12 on) has followed into the stage
-    const uint32_t last = __reduce_max_sync(0xffffffffu, issued);
-    for (uint32_t b = 0; b < 2 && j < kTileRecs && issued > b * kTileRecs; ++b) {
-      const uint32_t k = issued - 1 - b * kTileRecs;
-      if (k + kRawStages < last) break;
-      const unsigned long long t0 = global_ns();
-      while (!mbar_test(&sm.raw_full[k % kRawStages], (k / kRawStages) & 1) &&
-             global_ns() - t0 < kWaitLimitNs) {
-      }
-    }
-    __syncwarp();
+    // the copies still in flight land before the block ends
+    for (uint32_t k = groups > kGroups ? groups - kGroups : 0; k < groups; ++k)
+      mbar_wait(&sm.raw_full[k % kGroups], (k / kGroups) & 1, abort, false);
   };
 
   auto dequant_role = [&]() {
     const int dw = warp - kDequantWarp, g = lane >> 2, cc = lane & 3;
-    while (c.next(a, sm.pre, lane)) {
+    while (c.next(a, pre, lane)) {
       for (int i = 0; i < c.n; ++i, ++gi) {
         const int tok0 = (c.t0 + c.first + i) * kTileTok;
         bool skip[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const int j = dw + 4 * u;
-          const uint32_t k = gi * kTileRecs + j, st = k % kRawStages;
-          if (!mbar_wait(&sm.raw_full[st], (k / kRawStages) & 1, abort)) return;
-          skip[u] = sm.skip[st];
+          const uint32_t k = 2 * gi + u, st = k % kGroups;
+          if (!mbar_wait(&sm.raw_full[st], (k / kGroups) & 1, abort)) return;
+          skip[u] = sm.skip[st * kGroupRecs + dw];
         }
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
@@ -453,7 +444,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int j = dw + 4 * u;
-            const uint8_t* rec = sm.raw[(gi * kTileRecs + j) % kRawStages];
+            const uint8_t* rec = sm.raw[(2 * gi + u) % kGroups * kGroupRecs + dw];
             if (kv == 0 && lane == 0) {
               const float2 sc = *reinterpret_cast<const float2*>(rec + 32 * D);
               sm.scale[gi & 1][j] = skip[u] ? make_float4(0.f, -INFINITY, 0.f, 0.f)
@@ -498,8 +489,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
           if (lane == 0) {
             mbar_arrive(&sm.slot_full[slot]);
             if (kv == 1) {
-              mbar_arrive(&sm.raw_empty[(gi * kTileRecs + dw) % kRawStages]);
-              mbar_arrive(&sm.raw_empty[(gi * kTileRecs + dw + 4) % kRawStages]);
+              mbar_arrive(&sm.raw_empty[2 * gi % kGroups]);
+              mbar_arrive(&sm.raw_empty[(2 * gi + 1) % kGroups]);
             }
           }
         }
@@ -526,7 +517,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
       }
       __syncwarp();
     };
-    while (c.next(a, sm.pre, lane)) {
+    while (c.next(a, pre, lane)) {
       const int nt = c.tiles(a);
       for (int i = 0; i < c.n; ++i, ++gi) {
         const uint32_t ks = (2 * gi) % kSlots, ku = (2 * gi) / kSlots;
@@ -576,7 +567,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane 32 (warp % 4)
     const uint32_t ts = t * kTileTok + lanes, to = 2 * kTileTok + t * D + lanes;
     uint32_t n_s = 0, n_o = 0;
-    while (c.next(a, sm.pre, lane)) {
+    while (c.next(a, pre, lane)) {
       if (t >= c.tiles(a)) {
         gi += c.n;
         continue;
@@ -720,10 +711,10 @@ __global__ void __launch_bounds__(kTileJoinThreads) tile_join_kernel(AttnArgs a)
 
 template <int D, int KIND, typename T>
 static int launch_attend_tile(AttnArgs a, cudaStream_t st) {
-  const int smem = (int)(sizeof(TileSmem<D>) + a.v.B * sizeof(int32_t));
-  static_assert(sizeof(TileSmem<D>) + kMaxSeqs * sizeof(int32_t) <= 227 * 1024, "shared memory");
+  const int smem = (int)sizeof(TileSmem<D>);
+  static_assert(sizeof(TileSmem<D>) <= 227 * 1024, "shared memory");
   static std::atomic<uint64_t> done{0};
-  allow_smem(attend_tile_kernel<D, KIND, T>, 227 * 1024, done);
+  allow_smem(attend_tile_kernel<D, KIND, T>, smem, done);
   int rc = launch_next("paged_attention (tiles)", attend_tile_kernel<D, KIND, T>, dim3(kSms),
                        kTileThreads, smem, st, a);
   if (rc) return rc;
