@@ -29,6 +29,16 @@ constexpr int kMaxSeqs = 4096;                // sequences (or slots) per call
 enum Kind : int { kInt8 = 0, kE4m3 = 1 };
 enum StatusBit : int { kNoPages = 1, kBadSlot = 2 };  // bits of the page operations' status
 
+// Programmatic dependent launch: a kernel launched with that attribute may start
+// while the one before it in the stream still runs, and sees its writes only after
+// wait_previous(); let_next_start() allows the next such launch to begin.
+__device__ __forceinline__ void wait_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 __host__ __device__ constexpr int rec_bytes(int D) { return 32 * D + 16; }
 
 // The cache as one call sees it: a layer's pool, the page table and the call's
@@ -153,6 +163,12 @@ struct Code<kInt8> {
     auto q = [](float x) { return (uint32_t)(max(-127, min(127, __float2int_rn(x))) + 128); };
     return prmt(prmt(q(a), q(b), 0x0040), prmt(q(c), q(d), 0x0040), 0x5410);
   }
+  // The same for values that are known to be finite and at most 127.4: adding
+  // 1.5 * 2^23 + 128 rounds to nearest even and leaves the code in the low byte.
+  static __device__ __forceinline__ uint32_t pack_fine(float a, float b, float c, float d) {
+    auto q = [](float x) { return __float_as_uint(__fadd_rn(x, 12582912.f + 128.f)); };
+    return prmt(prmt(q(a), q(b), 0x0040), prmt(q(c), q(d), 0x0040), 0x5410);
+  }
   static __device__ __forceinline__ void unpack(uint32_t w, float (&x)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = (float)(int)((w >> (8 * e)) & 0xffu) - 128.f;
@@ -172,6 +188,13 @@ struct Code<kE4m3> {
     };
     return two(a, b) | (two(c, d) << 16);
   }
+  // The same without the care for NaN.
+  static __device__ __forceinline__ uint32_t pack_fine(float a, float b, float c, float d) {
+    uint16_t l, h;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(l) : "f"(b), "f"(a));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h) : "f"(d), "f"(c));
+    return (uint32_t)l | ((uint32_t)h << 16);
+  }
   static __device__ __forceinline__ void unpack(uint32_t w, float (&x)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; e += 2) {
@@ -183,6 +206,12 @@ struct Code<kE4m3> {
     }
   }
 };
+
+// Bits of the 16-bit infinity; a magnitude's bits order like the magnitude, NaN last.
+template <typename T>
+__device__ constexpr uint32_t inf_bits() {
+  return std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+}
 
 __device__ __forceinline__ float finite_abs(float x) {
   const float a = fabsf(x);
@@ -229,8 +258,86 @@ struct ValueMap {
 // Bound by HBM: 4 D bytes in and 2 D + 1 bytes out per token and head.
 constexpr int kAppendWarps = 4;
 
+// Largest finite magnitude of a lane's 16-byte words, over the warp; `fine`: all of
+// them are finite (else the slow way leaves the others out).
+template <int NC, typename T>
+__device__ __forceinline__ float warp_amax(const uint4 (&x)[NC], bool& fine) {
+  uint32_t mx = 0;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mx = __vmaxu2(mx, w[e] & 0x7fff7fffu);
+  }
+  mx = __reduce_max_sync(0xffffffffu, max(lo16(mx), hi16(mx)));
+  fine = mx < inf_bits<T>();
+  if (fine) return to_float2<T>(mx).x;
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 a = to_float2<T>(w[e]);
+      m = fmaxf(m, fmaxf(finite_abs(a.x), finite_abs(a.y)));
+    }
+  }
+  return warp_max(m);
+}
+
+// A lane's words of the new tokens as codes into the record. FINE: all finite.
+template <int D, int KIND, typename T, bool FINE>
+__device__ __forceinline__ void put_keys(const uint4 (&x)[D / 16], float inv, const KeyMap& km,
+                                         uint8_t* sm, int first, int last) {
+  using C = Code<KIND>;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    const int t = km.token(i);
+    const uint32_t xw[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const int ww = w ^ km.swap;
+      const float2 a = to_float2<T>(ww ? xw[2] : xw[0]), c = to_float2<T>(ww ? xw[3] : xw[1]);
+      const float y[4] = {__fmul_rn(a.x, inv), __fmul_rn(a.y, inv), __fmul_rn(c.x, inv),
+                          __fmul_rn(c.y, inv)};
+      const uint32_t code = FINE ? C::pack_fine(y[0], y[1], y[2], y[3])
+                                 : C::pack(y[0], y[1], y[2], y[3]);
+      if (first == 0 || (t >= first && t < last))
+        *reinterpret_cast<uint32_t*>(sm + km.offset(i, ww)) = code;
+    }
+  }
+}
+template <int D, int KIND, typename T, bool FINE>
+__device__ __forceinline__ void put_values(const uint4 (&x)[D / 16], float inv,
+                                           const ValueMap& vm, uint8_t* sm, int first, int last) {
+  using C = Code<KIND>;
+  uint32_t fresh = 0;  // bytes of a value word that are new tokens
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (vm.token(e) >= first && vm.token(e) < last) fresh |= 0xffu << (8 * e);
+#pragma unroll
+  for (int i = 0; i < D / 16; i += 4) {
+    const uint32_t* xw[4];
+#pragma unroll
+    for (int z = 0; z < 4; ++z) xw[z] = reinterpret_cast<const uint32_t*>(&x[i + z]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float y[4];
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        const float2 a = to_float2<T>(xw[z][e >> 1]);
+        y[z] = __fmul_rn((e & 1) ? a.y : a.x, inv);
+      }
+      const uint32_t code = FINE ? C::pack_fine(y[0], y[1], y[2], y[3])
+                                 : C::pack(y[0], y[1], y[2], y[3]);
+      uint32_t* at = reinterpret_cast<uint32_t*>(sm + 16 * D + vm.offset(i >> 2, e));
+      *at = first == 0 ? code : (*at & ~fresh) | (code & fresh);
+    }
+  }
+}
+
 template <int D, int KIND, typename T>
-__global__ void __launch_bounds__(32 * kAppendWarps) append_kernel(
+__global__ void __launch_bounds__(32 * kAppendWarps, 4) append_kernel(
     View v, const T* __restrict__ k, int64_t k_tok, int64_t k_head, const T* __restrict__ val,
     int64_t v_tok, int64_t v_head, int64_t n_warps) {
   constexpr int R = rec_bytes(D), NC = D / 16;  // NC: 16-byte words of a lane, K or V
@@ -238,6 +345,8 @@ __global__ void __launch_bounds__(32 * kAppendWarps) append_kernel(
   __shared__ __align__(128) uint8_t smem[kAppendWarps][(R + 127) / 128 * 128];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int64_t warp = (int64_t)blockIdx.x * kAppendWarps + wid;
+  wait_previous();
+  let_next_start();
   if (warp >= n_warps) return;
   const int h = (int)(warp % v.heads);
   int64_t b, local;
@@ -256,8 +365,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps) append_kernel(
   const int64_t blk64 = start / kBlock + local;
   if (local < 0 || blk64 * kBlock >= len) return;
   const int t0 = (int)blk64 * kBlock;
-  uint8_t* rec = v.record(s, (int)blk64, h);
-  if (!rec) return;
+  const int page = v.table[(int64_t)s * v.n_cols + blk64 / v.blocks];
   uint8_t* sm = smem[wid];
 
   // token t of the block is new when first <= t < last
@@ -267,7 +375,6 @@ __global__ void __launch_bounds__(32 * kAppendWarps) append_kernel(
   const KeyMap km(lane);
   const ValueMap vm(lane);
   uint4 kx[NC], vx[NC];
-  float ka = 0.f, va = 0.f;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int t = km.token(i);
@@ -279,103 +386,76 @@ __global__ void __launch_bounds__(32 * kAppendWarps) append_kernel(
     if (tv >= first && tv < last)
       vx[i] = *reinterpret_cast<const uint4*>(vp + tv * v_tok + vm.channel(i >> 2));
   }
-  float ks_old = 0.f, vs_old = 0.f;
-  if (first > 0) {
-    for (int o = lane * 16; o < R; o += 512)
-      *reinterpret_cast<uint4*>(sm + o) = *reinterpret_cast<const uint4*>(rec + o);
-    __syncwarp();
-    ks_old = *reinterpret_cast<const float*>(sm + 32 * D);
-    vs_old = *reinterpret_cast<const float*>(sm + 32 * D + 4);
+  if (page < 0 || page >= v.n_pages) {
+    atomicOr(&g_status, kStatusBadIndex);
+    return;
   }
+  uint8_t* rec =
+      v.pool + page * v.page_bytes() + h * v.head_bytes() + (blk64 % v.blocks) * (int64_t)R;
+  bool k_fine, v_fine;
+  float ks, vs, ki, vi;
+  if (first == 0) {
+    ks = fmaxf(__fmul_rn(warp_amax<NC, T>(kx, k_fine), 1.f / C::kMax), kScaleFloor);
+    vs = fmaxf(__fmul_rn(warp_amax<NC, T>(vx, v_fine), 1.f / C::kMax), kScaleFloor);
+    ki = __fdiv_rn(1.f, ks);
+    vi = __fdiv_rn(1.f, vs);
+  } else {
+    // An open block: a lane's 16-byte words of the record hold, for keys, tokens
+    // g and g + 8 in turn and, for values, the same four tokens in every word.
+    uint4 old[2 * (D / 32)];
 #pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const uint32_t kw[4] = {kx[i].x, kx[i].y, kx[i].z, kx[i].w};
-    const uint32_t vw[4] = {vx[i].x, vx[i].y, vx[i].z, vx[i].w};
+    for (int i = 0; i < 2 * (D / 32); ++i)
+      old[i] = *reinterpret_cast<const uint4*>(rec + 512 * i + 16 * lane);
+    const float2 sc = *reinterpret_cast<const float2*>(rec + 32 * D);
+    ks = fmaxf(sc.x, fmaxf(__fmul_rn(warp_amax<NC, T>(kx, k_fine), 1.f / C::kMax), kScaleFloor));
+    vs = fmaxf(sc.y, fmaxf(__fmul_rn(warp_amax<NC, T>(vx, v_fine), 1.f / C::kMax), kScaleFloor));
+    ki = __fdiv_rn(1.f, ks);
+    vi = __fdiv_rn(1.f, vs);
+    const uint32_t keep_k[2] = {(lane >> 2) < first ? ~0u : 0u, (lane >> 2) + 8 < first ? ~0u : 0u};
+    uint32_t keep_v = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 a = to_float2<T>(kw[e]), c = to_float2<T>(vw[e]);
-      ka = fmaxf(ka, fmaxf(finite_abs(a.x), finite_abs(a.y)));
-      va = fmaxf(va, fmaxf(finite_abs(c.x), finite_abs(c.y)));
-    }
-  }
-  const float ks = fmaxf(ks_old, fmaxf(__fmul_rn(warp_max(ka), 1.f / C::kMax), kScaleFloor));
-  const float vs = fmaxf(vs_old, fmaxf(__fmul_rn(warp_max(va), 1.f / C::kMax), kScaleFloor));
-  const float ki = __fdiv_rn(1.f, ks), vi = __fdiv_rn(1.f, vs);
-
-  if (first > 0) {
-    // older codes: restated when the scale grew; the places after them: 0
-    const float kf = __fmul_rn(ks_old, ki), vf = __fmul_rn(vs_old, vi);
-    for (int o = lane * 4; o < 32 * D; o += 128) {
-      uint32_t w = *reinterpret_cast<const uint32_t*>(sm + o);
-      const bool key = o < 16 * D;
-      if (key ? ks > ks_old : vs > vs_old) {
-        float x[4];
-        C::unpack(w, x);
-        const float f = key ? kf : vf;
-        w = C::pack(__fmul_rn(x[0], f), __fmul_rn(x[1], f), __fmul_rn(x[2], f),
-                    __fmul_rn(x[3], f));
+    for (int e = 0; e < 4; ++e)
+      if (2 * (lane & 3) + (e & 1) + 8 * (e >> 1) < first) keep_v |= 0xffu << (8 * e);
+#pragma unroll
+    for (int i = 0; i < 2 * (D / 32); ++i) {
+      const bool key = i < D / 32;
+      uint32_t w[4] = {old[i].x, old[i].y, old[i].z, old[i].w};
+      if (key ? ks > sc.x : vs > sc.y) {  // the scale grew: older codes anew
+        const float f = key ? __fmul_rn(sc.x, ki) : __fmul_rn(sc.y, vi);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x[4];
+          C::unpack(w[e], x);
+          w[e] = C::pack(__fmul_rn(x[0], f), __fmul_rn(x[1], f), __fmul_rn(x[2], f),
+                         __fmul_rn(x[3], f));
+        }
       }
-      uint32_t keep = 0;
-      if (key) {
-        keep = ((o >> 6) & 7) + 8 * ((o >> 2) & 1) < first ? 0xffffffffu : 0u;
-      } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (2 * ((o >> 4) & 3) + (e & 1) + 8 * (e >> 1) < first) keep |= 0xffu << (8 * e);
+      for (int e = 0; e < 4; ++e) {  // places after the older tokens: 0
+        const uint32_t keep = key ? keep_k[e & 1] : keep_v;
+        w[e] = (w[e] & keep) | (C::kZero & ~keep);
       }
-      *reinterpret_cast<uint32_t*>(sm + o) = (w & keep) | (C::kZero & ~keep);
+      *reinterpret_cast<uint4*>(sm + 512 * i + 16 * lane) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     __syncwarp();
   }
-
-#pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int t = km.token(i);
-    const uint32_t xw[4] = {kx[i].x, kx[i].y, kx[i].z, kx[i].w};
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const int ww = w ^ km.swap;
-      const uint32_t x0 = ww ? xw[2] : xw[0], x1 = ww ? xw[3] : xw[1];
-      const float2 a = to_float2<T>(x0), c = to_float2<T>(x1);
-      const uint32_t code = C::pack(__fmul_rn(a.x, ki), __fmul_rn(a.y, ki), __fmul_rn(c.x, ki),
-                                    __fmul_rn(c.y, ki));
-      if (first == 0 || (t >= first && t < last))
-        *reinterpret_cast<uint32_t*>(sm + km.offset(i, ww)) = code;
-    }
-  }
-  uint32_t fresh = 0;  // bytes of a value word that are new tokens
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (vm.token(e) >= first && vm.token(e) < last) fresh |= 0xffu << (8 * e);
-#pragma unroll
-  for (int i = 0; i < NC; i += 4) {
-    const uint32_t* x0 = reinterpret_cast<const uint32_t*>(&vx[i]);
-    const uint32_t* x1 = reinterpret_cast<const uint32_t*>(&vx[i + 1]);
-    const uint32_t* x2 = reinterpret_cast<const uint32_t*>(&vx[i + 2]);
-    const uint32_t* x3 = reinterpret_cast<const uint32_t*>(&vx[i + 3]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float2 a = to_float2<T>(x0[e >> 1]), bb = to_float2<T>(x1[e >> 1]);
-      const float2 c = to_float2<T>(x2[e >> 1]), d = to_float2<T>(x3[e >> 1]);
-      const uint32_t code =
-          (e & 1) ? C::pack(__fmul_rn(a.y, vi), __fmul_rn(bb.y, vi), __fmul_rn(c.y, vi),
-                            __fmul_rn(d.y, vi))
-                  : C::pack(__fmul_rn(a.x, vi), __fmul_rn(bb.x, vi), __fmul_rn(c.x, vi),
-                            __fmul_rn(d.x, vi));
-      uint32_t* at = reinterpret_cast<uint32_t*>(sm + 16 * D + vm.offset(i >> 2, e));
-      *at = first == 0 ? code : (*at & ~fresh) | (code & fresh);
-    }
-  }
-  if (lane < 4)
-    *reinterpret_cast<float*>(sm + 32 * D + 4 * lane) = lane == 0 ? ks : lane == 1 ? vs : 0.f;
+  if (k_fine) put_keys<D, KIND, T, true>(kx, ki, km, sm, first, last);
+  else put_keys<D, KIND, T, false>(kx, ki, km, sm, first, last);
+  if (v_fine) put_values<D, KIND, T, true>(vx, vi, vm, sm, first, last);
+  else put_values<D, KIND, T, false>(vx, vi, vm, sm, first, last);
   __syncwarp();
-  for (int o = lane * 16; o < R; o += 512)
-    *reinterpret_cast<uint4*>(rec + o) = *reinterpret_cast<const uint4*>(sm + o);
+#pragma unroll
+  for (int i = 0; i < 2 * (D / 32); ++i)
+    *reinterpret_cast<uint4*>(rec + 512 * i + 16 * lane) =
+        *reinterpret_cast<const uint4*>(sm + 512 * i + 16 * lane);
+  if (lane < 4) *reinterpret_cast<float*>(rec + 32 * D + 4 * lane) = lane == 0 ? ks : lane == 1 ? vs : 0.f;
 }
 
 // ---------------------------------------------------------------------------
 // Read: the tokens [starts[b], starts[b] + rows of b) of each sequence as 16-bit
-// or 32-bit values code * scale. One warp per (touched block, head).
+// or 32-bit values code * scale. One warp per touched block and `per_warp` heads:
+// four in large calls, which then hide the look-ups (indptr, length, table) behind
+// the records of the heads before.
 // ---------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&x)[8]);
@@ -401,16 +481,19 @@ template <int D, int KIND, typename T>
 __global__ void __launch_bounds__(32 * kAppendWarps) read_kernel(View v, const int32_t* starts,
                                                                  T* __restrict__ k,
                                                                  T* __restrict__ val,
-                                                                 int64_t n_warps) {
+                                                                 int64_t n_warps, int per_warp) {
   constexpr int R = rec_bytes(D), NC = D / 16;
   using C = Code<KIND>;
   __shared__ __align__(128) uint8_t smem[kAppendWarps][(R + 127) / 128 * 128];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int64_t warp = (int64_t)blockIdx.x * kAppendWarps + wid;
+  wait_previous();
+  let_next_start();
   if (warp >= n_warps) return;
-  const int h = (int)(warp % v.heads);
+  const int splits = (v.heads + per_warp - 1) / per_warp;
+  const int h0 = (int)(warp % splits) * per_warp, h1 = min(v.heads, h0 + per_warp);
   int64_t b, local;
-  find_item(v, warp / v.heads, lane, b, local);
+  find_item(v, warp / splits, lane, b, local);
   const int s = v.slot(b);
   if (s < 0) return;
   int64_t r0, r1;
@@ -424,44 +507,58 @@ __global__ void __launch_bounds__(32 * kAppendWarps) read_kernel(View v, const i
   }
   const int64_t blk = start / kBlock + local;
   if (local < 0 || blk * kBlock >= end) return;
-  const uint8_t* rec = v.record(s, (int)blk, h);
+  const uint8_t* rec = v.record(s, (int)blk, h0);
   if (!rec) return;
   uint8_t* sm = smem[wid];
-  for (int o = lane * 16; o < R; o += 512)
-    *reinterpret_cast<uint4*>(sm + o) = *reinterpret_cast<const uint4*>(rec + o);
-  __syncwarp();
-  const float ks = *reinterpret_cast<const float*>(sm + 32 * D);
-  const float vs = *reinterpret_cast<const float*>(sm + 32 * D + 4);
+  uint4 next[2 * (D / 32)];
+  float2 next_sc;
+  auto fetch = [&](int h) {
+    const uint8_t* p = rec + (h - h0) * v.head_bytes();
+#pragma unroll
+    for (int i = 0; i < 2 * (D / 32); ++i)
+      next[i] = *reinterpret_cast<const uint4*>(p + 512 * i + 16 * lane);
+    next_sc = *reinterpret_cast<const float2*>(p + 32 * D);
+  };
+  fetch(h0);
   const int64_t row0 = r0 + blk * kBlock - start;  // output row of the block's token 0
   const KeyMap km(lane);
   const ValueMap vm(lane);
+  for (int h = h0; h < h1; ++h) {
+    __syncwarp();
 #pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int64_t row = row0 + km.token(i);
-    float x[8];
+    for (int i = 0; i < 2 * (D / 32); ++i)
+      *reinterpret_cast<uint4*>(sm + 512 * i + 16 * lane) = next[i];
+    const float ks = next_sc.x, vs = next_sc.y;
+    if (h + 1 < h1) fetch(h + 1);
+    __syncwarp();
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      float y[4];
-      C::unpack(*reinterpret_cast<const uint32_t*>(sm + km.offset(i, w)), y);
+    for (int i = 0; i < NC; ++i) {
+      const int64_t row = row0 + km.token(i);
+      float x[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * w + e] = __fmul_rn(y[e], ks);
-    }
-    if (row >= r0 && row < r1) store8<T>(k + (row * v.heads + h) * D + km.channel(i), x);
-  }
+      for (int w = 0; w < 2; ++w) {
+        float y[4];
+        C::unpack(*reinterpret_cast<const uint32_t*>(sm + km.offset(i, w)), y);
 #pragma unroll
-  for (int i = 0; i < NC / 4; ++i) {
-    float x[4][8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float y[4];
-      C::unpack(*reinterpret_cast<const uint32_t*>(sm + 16 * D + vm.offset(i, e)), y);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) x[t][e] = __fmul_rn(y[t], vs);
+        for (int e = 0; e < 4; ++e) x[4 * w + e] = __fmul_rn(y[e], ks);
+      }
+      if (row >= r0 && row < r1) store8<T>(k + (row * v.heads + h) * D + km.channel(i), x);
     }
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int64_t row = row0 + vm.token(t);
-      if (row >= r0 && row < r1) store8<T>(val + (row * v.heads + h) * D + vm.channel(i), x[t]);
+    for (int i = 0; i < NC / 4; ++i) {
+      float x[4][8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float y[4];
+        C::unpack(*reinterpret_cast<const uint32_t*>(sm + 16 * D + vm.offset(i, e)), y);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[t][e] = __fmul_rn(y[t], vs);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int64_t row = row0 + vm.token(t);
+        if (row >= r0 && row < r1) store8<T>(val + (row * v.heads + h) * D + vm.channel(i), x[t]);
+      }
     }
   }
 }
@@ -786,6 +883,23 @@ __global__ void __launch_bounds__(kPageThreads) pairs_kernel(const int32_t* src,
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
+template <typename... Params, typename... Args>
+static int launch_next(const char* what, void (*kernel)(Params...), dim3 grid, int threads,
+                       int smem, cudaStream_t st, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, args...);
+  return check_launch(what);
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 inline int check_view(const char* what, const View& v, int kind, int page_tokens) {
@@ -861,18 +975,18 @@ static int launch_append(const View& v, const void* k, int64_t k_tok, int64_t k_
                          const void* val, int64_t v_tok, int64_t v_head, cudaStream_t st) {
   const int64_t warps = block_items(v) * v.heads;
   const int64_t grid = (warps + kAppendWarps - 1) / kAppendWarps;
-  append_kernel<D, KIND, T><<<(unsigned)grid, 32 * kAppendWarps, 0, st>>>(
-      v, (const T*)k, k_tok, k_head, (const T*)val, v_tok, v_head, warps);
-  return check_launch("paged_append");
+  return launch_next("paged_append", append_kernel<D, KIND, T>, dim3((unsigned)grid),
+                     32 * kAppendWarps, 0, st, v, (const T*)k, k_tok, k_head, (const T*)val, v_tok,
+                     v_head, warps);
 }
 
 template <int D, int KIND, typename T>
 static int launch_read(const View& v, const int32_t* starts, void* k, void* val, cudaStream_t st) {
-  const int64_t warps = block_items(v) * v.heads;
+  const int per_warp = block_items(v) * v.heads > 148 * 64 ? 4 : 1;
+  const int64_t warps = block_items(v) * ((v.heads + per_warp - 1) / per_warp);
   const int64_t grid = (warps + kAppendWarps - 1) / kAppendWarps;
-  read_kernel<D, KIND, T><<<(unsigned)grid, 32 * kAppendWarps, 0, st>>>(v, starts, (T*)k, (T*)val,
-                                                                       warps);
-  return check_launch("paged_read");
+  return launch_next("paged_read", read_kernel<D, KIND, T>, dim3((unsigned)grid),
+                     32 * kAppendWarps, 0, st, v, starts, (T*)k, (T*)val, warps, per_warp);
 }
 
 inline int move_grid() { return 148 * 4; }

@@ -365,16 +365,6 @@ __device__ __forceinline__ float2 row_stats(float m, float m2, float l) {
   return make_float2(m * kLn2, __fdiv_rn(1.f, l * exp2f(m2 - m)));
 }
 
-// Programmatic dependent launch: a kernel launched with that attribute may start
-// while the one before it in the stream still runs, and sees its writes only after
-// wait_previous(); let_next_start() allows the next such launch to begin.
-__device__ __forceinline__ void wait_previous() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-__device__ __forceinline__ void let_next_start() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
 // 8 consumer warps, and 4 that feed two each. A copy is issued for one lane at a time
 // (~190 cycles each), so one warp that fed all eight was what bound the kernel: 1500
 // cycles for 8 records, the rate of HBM itself (16 x 5 rows, window 2500: 55 us).
@@ -815,23 +805,6 @@ static void allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) ==
       cudaSuccess)
     done.fetch_or(bit, std::memory_order_relaxed);
-}
-
-template <typename... Params, typename... Args>
-static int launch_next(const char* what, void (*kernel)(Params...), dim3 grid, int threads,
-                       int smem, cudaStream_t st, const Args&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kernel, args...);
-  return check_launch(what);
 }
 
 template <int D, int KIND, int NT, typename T>
