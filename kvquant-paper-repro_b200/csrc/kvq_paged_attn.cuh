@@ -121,8 +121,8 @@ __device__ __forceinline__ Seq load_seq(const AttnArgs& a, int64_t b, int R,
 // Work is a flat sequence of 16-token blocks over (sequence, head, row group),
 // and worker w of W takes an equal share of it, whatever the lengths are. Each
 // unit counts kUnitCost blocks more than it has, its first places: starting and
-// ending a unit takes a warp about that long (2 us against 0.84 us a block), and
-// workers with many short sequences ended 6 us after the others without it.
+// ending one takes a warp about 2 us, a block 0.84 us. (Batches of 16 ragged
+// sequences measure the same with and without; it is for many short ones.)
 // pre[b] = places of the sequences before b, per head. Block-wide; pre has B + 1.
 constexpr int kUnitCost = 2;
 template <int THREADS>
@@ -367,7 +367,8 @@ __device__ __forceinline__ float2 row_stats(float m, float m2, float l) {
 
 // 8 consumer warps, and 4 that feed two each. A copy is issued for one lane at a time
 // (~190 cycles each), so one warp that fed all eight was what bound the kernel: 1500
-// cycles for 8 records, the rate of HBM itself (16 x 5 rows, window 2500: 55 us).
+// cycles for 8 records, the rate of HBM itself (262144 tokens x 32 heads: 370 us with
+// one, 315 with four).
 constexpr int kAttnWarps = 8, kFeeds = 2;
 constexpr int kAttnThreads = 32 * (kAttnWarps + kAttnWarps / kFeeds);
 constexpr int kSms = 148;
@@ -424,8 +425,10 @@ struct Cursor {
 // One CTA per SM. Every consumer warp works through its own share of the blocks
 // with its own ring of records, so no warp waits for another one; a lane of a
 // feeding warp keeps each ring full: one bulk copy per record, on across the ends of
-// units. 8 warps hide the ~500 cycles a block takes a warp
-// (HBM delivers one per ~180 cycles and SM).
+// units. Bound by HBM: 262144 tokens x 32 heads, 2.16 GB, take 315 us = 6.8 TB/s (of a
+// measured copy rate of 6.55); 16 sequences of up to 8192, 0.145 GB, 37 us, of which
+// ~7 pass before the first record, ~5 in the join, and the last SM ends ~5 after the
+// median one.
 template <int D, int KIND, int NT, typename T>
 __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
   constexpr int R = 8 * NT, S = Ring<D>::kStages;
@@ -786,8 +789,8 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttnArgs a, i
 
 // Rows of a call's largest sequence: 8-row tiles where one is enough, up to three
 // groups of two, else (0) the 128-row tiles of kvq_paged_tile.cuh. 23 sequences of up
-// to 6000 tokens, window 2500, D = 64 / 128: 48 rows 84 / 107 us in groups against
-// 101 / 136 in tiles, 64 rows 108 / 137 against 102 / 140; one of 32768 tokens: 32
+// to 6000 tokens, window 2500, D = 64 / 128: 48 rows 75 / 109 us in groups against
+// 101 / 136 in tiles, 64 rows 108 / 137 against 102 / 141; one of 32768 tokens: 32
 // rows 51 against 62, 64 rows 77 against 65.
 constexpr int kGroupRows = 48;
 inline int row_tiles(int64_t max_new, int64_t group) {
