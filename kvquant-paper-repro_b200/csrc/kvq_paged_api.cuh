@@ -47,13 +47,13 @@ extern "C" int kvq_paged_attention(const void* q, int64_t q_tok_stride, int64_t 
               (long long)n_heads);
     return KVQ_ERR_UNSUPPORTED;
   }
-  if (max_new < 0 || max_new > 65536 || (!indptr && max_new < total / B) || window < 0 ||
+  if (max_new < (total > 0) || max_new > 65536 || (!indptr && max_new < total / B) || window < 0 ||
       window > INT32_MAX) {
-    set_error("paged_attention: max_new %lld (0..65536, at least the rows a sequence) or window "
+    set_error("paged_attention: max_new %lld (1..65536, at least the rows a sequence) or window "
               "%lld", (long long)max_new, (long long)window);
     return KVQ_ERR_INVALID;
   }
-  if (total == 0 || max_new == 0) return KVQ_OK;
+  if (total == 0) return KVQ_OK;
   if (!q || !out || !aligned16(q) || q_tok_stride % 8 || q_head_stride % 8 ||
       (reinterpret_cast<uintptr_t>(out) & 15) || (reinterpret_cast<uintptr_t>(ml_out) & 7)) {
     set_error("paged_attention: q rows and out must be 16-byte aligned (strides multiples of 8), "

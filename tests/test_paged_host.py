@@ -94,7 +94,7 @@ def test_cache_arguments_are_checked(lib, call, kw, rc, what):
     (append, dict(v=ctypes.c_void_p(8)), 1, b"aligned"), (append, dict(kt=132), 1, b"strides"),
     (attend, dict(dtype=2), 3, b"dtype"), (attend, dict(group=65), 3, b"query heads"),
     (attend, dict(group=0), 3, b"query heads"), (attend, dict(max_new=0), 1, b"max_new"),
-    (attend, dict(window=-1), 1, b"window"), (attend, dict(q=None), 1, b"aligned"),
+    (attend, dict(max_new=0, ip=P), 1, b"max_new"), (attend, dict(window=-1), 1, b"window"), (attend, dict(q=None), 1, b"aligned"),
     (attend, dict(out=ctypes.c_void_p(8)), 1, b"aligned"), (attend, dict(wsb=64), 1, b"workspace"),
     (attend, dict(ws=None), 1, b"workspace"), (attend, dict(ml=ctypes.c_void_p(4)), 1, b"aligned"),
     (read, dict(dtype=3), 3, b"dtype"), (read, dict(k=None), 1, b"aligned"),
