@@ -6,13 +6,18 @@
 //   t_j = (q . kcode_j) ks_b scale log2(e)            (b the block of token j)
 //   p_j = 2^(t_j - m), out = sum_j p_j vs_b vcode_j / sum_j p_j
 // over the tokens j <= position, j > position - window. The value scale joins
-// the exponent: w_j = 2^(t_j + log2 vs_b - m2) <= 1 with m2 the running maximum
-// of the exponents, so that the fp16 weights of the second product are relative
-// to the largest contribution whatever the blocks' scales are; the softmax sum
-// is sum_j w_j / vs_b in the same reference, out = O / that. Codes are exact in
-// fp16 (8 bits), fp16 queries too, and bf16 queries once a row is scaled by a
-// power of two; products and sums are fp32. The only roundings to fewer bits
-// are w_j (fp16, relative 2^-12, or 2^-25 of the largest) and the output.
+// the exponent: w_j = 2^(t_j + log2 vs_b - m2 + lift) with m2 the running maximum
+// of t_j + log2 vs_b, so that the fp16 weights of the second product are relative
+// to the largest contribution p_j vs_b; the softmax sum is sum_j w_j / vs_b in the
+// same reference, out = O / that. The lift puts the largest weight at 2^15, near
+// fp16's end: weights are normal numbers down to 2^-29 of it and steps of 2^-39
+// below (2^-25 and 2^-35 in the kernel of many rows, whose m2 may lag behind), so
+// a block whose scale one large channel sets leaves the others' weights their
+// bits; only where scales differ by more do the smaller blocks lose them. Codes are
+// exact in fp16 (8 bits), fp16 queries too, and bf16 queries once a row is scaled
+// by a power of two (elements below 2^-31 of their row's largest lose bits);
+// products and sums are fp32. The only other roundings to fewer bits are w_j
+// (fp16, relative 2^-12) and the output.
 #pragma once
 #include <atomic>
 
@@ -23,6 +28,7 @@ namespace paged {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLift = 15.f;  // log2 of the largest weight (fp16 ends at 65504)
 
 struct AttnArgs {
   View v;
@@ -298,8 +304,9 @@ __device__ __forceinline__ void block_step(State<D, NT>& st, const uint8_t* cons
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
       const float was = st.m2[t][r], now = fmaxf(was, top);
       grew |= now > was;
-      ref[r] = now == -INFINITY ? 0.f : now;
-      alpha[r] = exp2_approx(was - ref[r]);
+      const float base = now == -INFINITY ? 0.f : now;
+      ref[r] = base - kLift;
+      alpha[r] = exp2_approx(was - base);
       st.m2[t][r] = now;
     }
     if (__any_sync(0xffffffffu, grew)) {
@@ -359,10 +366,11 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) {
   return __float2bfloat16_rn(x);
 }
 
-// (max, 1 / sum) of a row in natural units; a row that sees nothing has (-inf, inf).
-__device__ __forceinline__ float2 row_stats(float m, float m2, float l) {
+// (max, 1 / sum) of a row in natural units, from the maximum of its scores and its sum
+// relative to 2^ref (both in log2 units); a row that sees nothing has (-inf, inf).
+__device__ __forceinline__ float2 row_stats(float m, float ref, float l) {
   if (l == 0.f) return make_float2(-INFINITY, INFINITY);
-  return make_float2(m * kLn2, __fdiv_rn(1.f, l * exp2f(m2 - m)));
+  return make_float2(m * kLn2, __fdiv_rn(1.f, l * exp2f(ref - m)));
 }
 
 // 8 consumer warps, and 4 that feed two each. A copy is issued for one lane at a time
@@ -624,7 +632,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
             out[16 * i + g] = from_float<T>(st.o[i][t][r] * inv);
             out[16 * i + 8 + g] = from_float<T>(st.o[i][t][r + 2] * inv);
           }
-          if (a.ml && g == 0) a.ml[at] = row_stats(st.m[t][r], st.m2[t][r], st.l[t][r]);
+          if (a.ml && g == 0) a.ml[at] = row_stats(st.m[t][r], st.m2[t][r] - kLift, st.l[t][r]);
         } else {
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) {
@@ -715,17 +723,17 @@ __device__ __forceinline__ void join_row(int n, int part, int split, int rows, i
   }
 }
 
-// A joined row's output and statistics (l: the whole sum).
+// A joined row's output and statistics (l: the whole sum, relative to 2^ref).
 template <int D, typename T>
 __device__ __forceinline__ void store_row(const AttnArgs& a, int64_t at, int lane,
-                                          const float (&o)[D / 32], float m, float m2, float l) {
+                                          const float (&o)[D / 32], float m, float ref, float l) {
   const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
   T* out = (T*)a.out + at * D + D / 32 * lane;
 #pragma unroll
   for (int e = 0; e < D / 32; e += 2)
     *reinterpret_cast<uint32_t*>(out + e) =
         l == 0.f ? 0u : from_float2<T>(o[e] * inv, o[e + 1] * inv);
-  if (a.ml && lane == 0) a.ml[at] = row_stats(m, m2, l);
+  if (a.ml && lane == 0) a.ml[at] = row_stats(m, ref, l);
 }
 
 // Joins the pieces of the units that several workers share, in a fixed order. A
@@ -784,7 +792,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttnArgs a, i
   if (n == 0) return;
   const int64_t at = (s.r0 + row / a.group) * ((int64_t)a.v.heads * a.group) + h * a.group +
                      row % a.group;
-  store_row<D, T>(a, at, lane, o, m, m2, l);
+  store_row<D, T>(a, at, lane, o, m, m2 - kLift, l);
 }
 
 // Rows of a call's largest sequence: 8-row tiles where one is enough, up to three

@@ -36,7 +36,10 @@ constexpr int kRegsSoftmax = 192, kRegsDequant = 80, kRegsIssue = 48;
 static_assert(2 * kRegsSoftmax + kRegsDequant + kRegsIssue <= 4 * 128, "register shares");
 constexpr int kDequantWarp = 8, kMmaWarp = 12, kLoadWarp = 13;
 constexpr int64_t kTileParts = 2 * kSms;  // pieces in the workspace, then B + 1 int32
-constexpr float kLazy = 8.f;  // the maximum may grow by 2^8 before O is rescaled
+// The maximum may grow by 2^kLazy before O is rescaled, and weights are lifted by that
+// much less: together 2^15.875, below fp16's end. (Two chunks of 2048 tokens: 728 us at 8
+// without a lift, 767 at 4; what a rescaling costs is a pass over O in TMEM.)
+constexpr float kTileLift = 11.f, kLazy = 4.875f;
 
 template <int D>
 struct TileSmem {
@@ -319,7 +322,7 @@ __device__ __forceinline__ void softmax_tile(RowState& st, uint32_t ts, uint32_t
       }
     }
   }
-  const float base = st.ref == -INFINITY ? 0.f : st.ref;
+  const float base = (st.ref == -INFINITY ? 0.f : st.ref) - kTileLift;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     uint32_t p[16];
@@ -640,7 +643,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
         }
       }
       if (valid && whole) {
-        if (a.ml) a.ml[at] = row_stats(st.m, st.ref, l);
+        if (a.ml) a.ml[at] = row_stats(st.m, st.ref - kTileLift, l);
       } else if (valid) {
         *reinterpret_cast<float4*>(part + kUnitRows * D + 4 * ur) = make_float4(st.ref, l, st.m, 0.f);
       }
@@ -709,7 +712,7 @@ __global__ void __launch_bounds__(kTileJoinThreads) tile_join_kernel(AttnArgs a)
     l = warp_sum(l);
     const int64_t at = (c.s.r0 + r / a.group) * ((int64_t)a.v.heads * a.group) +
                        c.h * a.group + r % a.group;
-    store_row<D, T>(a, at, lane, o, m, ref, l);
+    store_row<D, T>(a, at, lane, o, m, ref - kTileLift, l);
   }
 }
 
