@@ -83,6 +83,12 @@ __device__ __forceinline__ void code_halves(uint32_t w, uint32_t& lo, uint32_t& 
   }
 }
 
+// First token that a row at `pos` sees. A row before the first token (pos < 0) sees none,
+// whatever this says; windows reach INT32_MAX, so pos is clamped before it is subtracted.
+__device__ __forceinline__ int first_seen(int pos, int window) {
+  return window > 0 ? max(0, max(pos, 0) - window + 1) : 0;
+}
+
 // What one call sees of sequence b. A row group is R = 8 * NT query rows (token,
 // query head of the KV head's group), row r being token r / group.
 struct Seq {
@@ -99,8 +105,7 @@ __device__ __forceinline__ Seq make_seq(const AttnArgs& a, int slot, int len, in
   s.len = len;
   s.n = n;
   s.r0 = r0;
-  const int lo = a.window > 0 ? max(0, len - n - a.window + 1) : 0;
-  s.lo_blk = lo / kBlock;
+  s.lo_blk = first_seen(len - n, a.window) / kBlock;
   // an empty sequence still has a (wholly masked) block, which writes its rows
   s.n_blk = n == 0 ? 0 : max(1, (len + kBlock - 1) / kBlock - s.lo_blk);
   s.groups = (int)(((int64_t)n * a.group + R - 1) / R);
@@ -568,12 +573,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
       for (int r = 0; r < 2; ++r) {
         const int row = row0 + 8 * t + 2 * c + r, pos = s.len - s.n + row / a.group;
         hi[t][r] = row < rows ? pos : -1;
-        lo[t][r] = a.window > 0 ? pos - a.window + 1 : 0;
+        lo[t][r] = first_seen(pos, a.window);
       }
     // tokens [see_lo, see_hi] are visible to every row of the group
     const int see_hi = s.len - s.n + row0 / a.group;
     const int last = s.len - s.n + (min(row0 + R, rows) - 1) / a.group;
-    const int see_lo = a.window > 0 ? last - a.window + 1 : 0;
+    const int see_lo = first_seen(last, a.window);
     State<D, NT> st;
     st.clear();
     auto visible = [&](int t0) { return t0 >= see_lo && t0 + kBlock - 1 <= see_hi; };

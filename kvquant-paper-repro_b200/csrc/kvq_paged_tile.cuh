@@ -62,7 +62,7 @@ __device__ __forceinline__ void unit_tiles(const AttnArgs& a, const Seq& s, int 
   const int p0 = s.len - s.n + (int)((int64_t)r * kUnitRows / a.group);
   const int p1 = s.len - s.n +
                  min(s.n - 1, (int)(((int64_t)r * kUnitRows + kUnitRows - 1) / a.group));
-  t0 = a.window > 0 ? max(0, p0 - a.window + 1) / kTileTok : 0;
+  t0 = first_seen(p0, a.window) / kTileTok;
   n = max(1, max(p1, 0) / kTileTok - t0 + 1);
 }
 
@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(AttnArgs a
       int lo = 0;
       uint32_t span = INT_MAX;
       if (valid) {
-        lo = pos < 0 ? INT_MAX : a.window > 0 ? max(0, pos - a.window + 1) : 0;
+        lo = pos < 0 ? INT_MAX : first_seen(pos, a.window);
         span = pos < 0 ? 0 : pos - lo;
       }
       const bool idle = !__any_sync(0xffffffffu, valid);
