@@ -889,10 +889,8 @@ __global__ void __launch_bounds__(kPageThreads) pairs_kernel(const int32_t* src,
                                                              int64_t n, Moves* moves, int2* list) {
   wait_previous();
   let_next_start();
-  __shared__ int kept;
   __shared__ int warp_sums[32];
-  if (threadIdx.x == 0) kept = 0;
-  __syncthreads();
+  int kept = 0;  // the same in every thread
   for (int64_t i0 = 0; i0 < n; i0 += kPageThreads) {
     const int64_t i = i0 + threadIdx.x;
     bool ok = i < n;
@@ -904,10 +902,9 @@ __global__ void __launch_bounds__(kPageThreads) pairs_kernel(const int32_t* src,
       if (!ok) atomicOr(&g_status, kStatusBadIndex);
     }
     int sum;
-    const int at = kept + block_scan(ok, warp_sums, sum);
-    if (ok) list[at] = make_int2(a, c);
-    if (threadIdx.x == 0) kept += sum;
-    __syncthreads();
+    const int at = block_scan(ok, warp_sums, sum);
+    if (ok) list[kept + at] = make_int2(a, c);
+    kept += sum;
   }
   if (threadIdx.x == 0) moves->count = kept;
 }

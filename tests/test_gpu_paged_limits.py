@@ -22,3 +22,24 @@ def test_windows_that_hide_nothing(cuda, window, max_new):
     assert (out[:3] == 0).all() and np.isneginf(ml[:3, :, 0]).all()
     check(out, e_out, b_out, "out")
     check(ml, e_ml, b_ml, "ml")
+
+
+@pytest.mark.parametrize("n", [255, 256, 257, 1000])
+def test_copy_of_many_pages(cuda, n):
+    """Lists longer than one scan of the planning block, with pairs out of range among them."""
+    from kvquant.kernels import paged_copy
+    from kvquant.kernels.cuda_ops import get_cuda_ops
+    rng = np.random.default_rng(n)
+    a, b = (rng.integers(0, 256, (2, n + 3, 1, 1, 32 * 64 + 16), dtype=np.uint8) for _ in range(2))
+    src, dst = (rng.integers(0, n + 3, n), rng.permutation(n + 3)[:n])
+    bad = rng.random(n) < 0.1
+    src[bad & (rng.random(n) < 0.5)] = -1
+    dst[bad & (src >= 0)] = n + 3
+    t = lambda x: torch.from_numpy(np.ascontiguousarray(x)).to(cuda)  # noqa: E731
+    ga, gb = t(a), t(b)
+    paged_copy(ga, gb, t(src.astype(np.int32)), t(dst.astype(np.int32)))
+    with pytest.raises(RuntimeError, match="out of range"):
+        get_cuda_ops().check_status(cuda)
+    b[:, dst[~bad]] = a[:, src[~bad]]
+    np.testing.assert_array_equal(gb.cpu().numpy(), b)
+    np.testing.assert_array_equal(ga.cpu().numpy(), a)
