@@ -381,6 +381,17 @@ int kvq_paged_append(const void* k, int64_t k_tok_stride, int64_t k_head_stride,
                      const int32_t* lengths, const int32_t* slots, const int32_t* indptr,
                      int64_t B, int64_t total, void* stream);
 
+/* The same, with granted: int32 [n_slots] as kvq_paged_extend_granting keeps it. A
+ * sequence with rows before granted[slot] is skipped and flagged, so an append after
+ * a refused extend leaves the stored tokens alone. */
+int kvq_paged_append_granted(const void* k, int64_t k_tok_stride, int64_t k_head_stride,
+                             const void* v, int64_t v_tok_stride, int64_t v_head_stride, int dtype,
+                             uint8_t* pool, int kind, int64_t n_pages, int64_t n_heads,
+                             int64_t head_dim, int64_t page_tokens, const int32_t* table,
+                             int64_t n_slots, int64_t n_cols, const int32_t* lengths,
+                             const int32_t* slots, const int32_t* indptr, int64_t B, int64_t total,
+                             const int32_t* granted, void* stream);
+
 /* Values of the tokens [starts[b], starts[b] + rows of b) (starts NULL: 0) as
  * k_out, v_out [total, n_heads, D] of `dtype`. */
 int kvq_paged_read(const uint8_t* pool, int kind, int64_t n_pages, int64_t n_heads,
@@ -431,6 +442,17 @@ int kvq_paged_extend(uint8_t* pool, int64_t n_layers, int64_t layer_stride, int6
                      int32_t* refs, int64_t n_pages, int64_t page_tokens, const int32_t* slots,
                      int64_t n, const int32_t* n_new, int64_t n_new_all, int32_t* status,
                      void* workspace, size_t workspace_bytes, void* stream);
+/* The same, and granted: int32 [n_slots] (device) gets the first new token of each of
+ * the slots, INT32_MAX when the call is refused. Without it, nothing on the device
+ * keeps an append after a refused extend from the slots' last stored tokens: the
+ * caller has to read status first. */
+int kvq_paged_extend_granting(uint8_t* pool, int64_t n_layers, int64_t layer_stride,
+                              int64_t page_bytes, int32_t* table, int64_t n_slots, int64_t n_cols,
+                              int32_t* lengths, int32_t* refs, int64_t n_pages,
+                              int64_t page_tokens, const int32_t* slots, int64_t n,
+                              const int32_t* n_new, int64_t n_new_all, int32_t* status,
+                              void* workspace, size_t workspace_bytes, int32_t* granted,
+                              void* stream);
 /* compact: with L live pages (refs > 0), those with ids >= L move in ascending
  * order into the free ids below L, in every layer; table and refs follow, L goes
  * to *n_live (device). Workspace: kvq_paged_extend_workspace(n_pages). */

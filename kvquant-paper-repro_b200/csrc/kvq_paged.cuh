@@ -255,6 +255,8 @@ struct ValueMap {
 // an open block keeps the larger of its scale and that, and its older codes are
 // restated as round(code * s_old / s) when it grew: at most half a step of the
 // new scale of error each time. Places past the last token hold the code 0.
+// granted: the first token of each slot that its last extend granted (null: not kept);
+// tokens before it are stored already, perhaps for several slots, and are not written over.
 // Bound by HBM: 4 D bytes in and 2 D + 1 bytes out per token and head. 17 prompts, 8
 // heads, D = 128, bf16 to e4m3: 41 us for 0.21 GB = 5.1 TB/s (128 registers, 16 warps an
 // SM); one token of 64 sequences: 5 us, five dependent look-ups.
@@ -341,7 +343,7 @@ __device__ __forceinline__ void put_values(const uint4 (&x)[D / 16], float inv,
 template <int D, int KIND, typename T>
 __global__ void __launch_bounds__(32 * kAppendWarps, 4) append_kernel(
     View v, const T* __restrict__ k, int64_t k_tok, int64_t k_head, const T* __restrict__ val,
-    int64_t v_tok, int64_t v_head, int64_t n_warps) {
+    int64_t v_tok, int64_t v_head, const int32_t* granted, int64_t n_warps) {
   constexpr int R = rec_bytes(D), NC = D / 16;  // NC: 16-byte words of a lane, K or V
   using C = Code<KIND>;
   __shared__ __align__(128) uint8_t smem[kAppendWarps][(R + 127) / 128 * 128];
@@ -360,7 +362,8 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 4) append_kernel(
   const int len = v.length(s);
   const int start = len - (int)(r1 - r0);
   if (r1 == r0) return;
-  if (start < 0) {  // more new tokens than the slot holds
+  // more new tokens than the slot holds, or than it was granted
+  if (start < 0 || (granted && start < granted[s])) {
     atomicOr(&g_status, kStatusBadIndex);
     return;
   }
@@ -672,13 +675,13 @@ struct Moves {
 // One CTA: pages for the new tokens of every slot, taken from the free ones in
 // ascending order, slot after slot in the list's order. A slot whose last page
 // is open and shared gets a page of its own for it (to be copied by
-// move_kernel) unless every other holder stands before it in the list. Nothing
-// changes when the call is refused.
+// move_kernel) unless every other holder stands before it in the list. When the
+// call is refused nothing changes but `granted`: no token of its slots is.
 __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Meta m, const int32_t* slots,
                                                               int64_t n, const int32_t* n_new,
                                                               int n_new_all, int32_t* status,
                                                               Moves* moves, int2* list,
-                                                              int32_t* pages) {
+                                                              int32_t* pages, int32_t* granted) {
   wait_previous();
   let_next_start();
   __shared__ int warp_sums[32];
@@ -686,6 +689,14 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Meta m, const int3
   __shared__ int need[kMaxSeqs];       // pages, then its offset; copy flag in `copies`
   __shared__ uint8_t copies[kMaxSeqs];
   const int tid = threadIdx.x;
+  auto refuse = [&](int why) {
+    for (int64_t i = tid; granted && i < n; i += kPlanThreads)
+      if (slots[i] >= 0 && slots[i] < m.n_slots) granted[slots[i]] = INT32_MAX;
+    if (tid == 0) {
+      atomicOr(status, why);
+      moves->count = 0;
+    }
+  };
   int bad = 0;
   for (int i = tid; i < n; i += kPlanThreads) {
     const int s = slots[i], add = n_new ? n_new[i] : n_new_all;
@@ -721,10 +732,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Meta m, const int3
   }
   bad = __syncthreads_or(bad);
   if (bad) {
-    if (tid == 0) {
-      atomicOr(status, kBadSlot);
-      moves->count = 0;
-    }
+    refuse(kBadSlot);
     return;
   }
   int total = 0;
@@ -750,10 +758,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Meta m, const int3
     found += sum;
   }
   if (found < total) {
-    if (tid == 0) {
-      atomicOr(status, kNoPages);
-      moves->count = 0;
-    }
+    refuse(kNoPages);
     return;
   }
   __syncthreads();
@@ -781,6 +786,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Meta m, const int3
     if (lane == 0) {
       if (copies[i]) atomicSub(&m.refs[last_page[i]], 1);
       m.lengths[s] = (int)(len + add);
+      if (granted) granted[s] = (int)len;
     }
   }
 }
@@ -1001,12 +1007,13 @@ inline View make_view(uint8_t* pool, int64_t n_pages, int64_t heads, int64_t dim
 
 template <int D, int KIND, typename T>
 static int launch_append(const View& v, const void* k, int64_t k_tok, int64_t k_head,
-                         const void* val, int64_t v_tok, int64_t v_head, cudaStream_t st) {
+                         const void* val, int64_t v_tok, int64_t v_head, const int32_t* granted,
+                         cudaStream_t st) {
   const int64_t warps = block_items(v) * v.heads;
   const int64_t grid = (warps + kAppendWarps - 1) / kAppendWarps;
   return launch_next("paged_append", append_kernel<D, KIND, T>, dim3((unsigned)grid),
                      32 * kAppendWarps, 0, st, v, (const T*)k, k_tok, k_head, (const T*)val, v_tok,
-                     v_head, warps);
+                     v_head, granted, warps);
 }
 
 template <int D, int KIND, typename T>
@@ -1049,6 +1056,20 @@ extern "C" int kvq_paged_append(const void* k, int64_t k_tok_stride, int64_t k_h
                                 const int32_t* table, int64_t n_slots, int64_t n_cols,
                                 const int32_t* lengths, const int32_t* slots,
                                 const int32_t* indptr, int64_t B, int64_t total, void* stream) {
+  return kvq_paged_append_granted(k, k_tok_stride, k_head_stride, v, v_tok_stride, v_head_stride,
+                                  dtype, pool, kind, n_pages, n_heads, head_dim, page_tokens,
+                                  table, n_slots, n_cols, lengths, slots, indptr, B, total,
+                                  nullptr, stream);
+}
+
+extern "C" int kvq_paged_append_granted(const void* k, int64_t k_tok_stride, int64_t k_head_stride,
+                                        const void* v, int64_t v_tok_stride, int64_t v_head_stride,
+                                        int dtype, uint8_t* pool, int kind, int64_t n_pages,
+                                        int64_t n_heads, int64_t head_dim, int64_t page_tokens,
+                                        const int32_t* table, int64_t n_slots, int64_t n_cols,
+                                        const int32_t* lengths, const int32_t* slots,
+                                        const int32_t* indptr, int64_t B, int64_t total,
+                                        const int32_t* granted, void* stream) {
   using namespace kvq;
   using namespace kvq::paged;
   clear_error();
@@ -1072,7 +1093,8 @@ extern "C" int kvq_paged_append(const void* k, int64_t k_tok_stride, int64_t k_h
   }
   const cudaStream_t st = as_stream(stream);
 #define KVQ_PAGED_APPEND(D, KIND, T) \
-  launch_append<D, KIND, T>(w, k, k_tok_stride, k_head_stride, v, v_tok_stride, v_head_stride, st)
+  launch_append<D, KIND, T>(w, k, k_tok_stride, k_head_stride, v, v_tok_stride, v_head_stride, \
+                            granted, st)
 #define KVQ_PAGED_PICK(D, T) \
   (kind == kInt8 ? KVQ_PAGED_APPEND(D, kInt8, T) : KVQ_PAGED_APPEND(D, kE4m3, T))
   if (head_dim == 64)
@@ -1169,6 +1191,18 @@ extern "C" int kvq_paged_extend(uint8_t* pool, int64_t n_layers, int64_t layer_s
                                 int64_t page_tokens, const int32_t* slots, int64_t n,
                                 const int32_t* n_new, int64_t n_new_all, int32_t* status,
                                 void* workspace, size_t workspace_bytes, void* stream) {
+  return kvq_paged_extend_granting(pool, n_layers, layer_stride, page_bytes, table, n_slots, n_cols,
+                                   lengths, refs, n_pages, page_tokens, slots, n, n_new, n_new_all,
+                                   status, workspace, workspace_bytes, nullptr, stream);
+}
+
+extern "C" int kvq_paged_extend_granting(uint8_t* pool, int64_t n_layers, int64_t layer_stride,
+                                         int64_t page_bytes, int32_t* table, int64_t n_slots,
+                                         int64_t n_cols, int32_t* lengths, int32_t* refs,
+                                         int64_t n_pages, int64_t page_tokens,
+                                         const int32_t* slots, int64_t n, const int32_t* n_new,
+                                         int64_t n_new_all, int32_t* status, void* workspace,
+                                         size_t workspace_bytes, int32_t* granted, void* stream) {
   using namespace kvq;
   using namespace kvq::paged;
   clear_error();
@@ -1199,7 +1233,7 @@ extern "C" int kvq_paged_extend(uint8_t* pool, int64_t n_layers, int64_t layer_s
   int32_t* pages = reinterpret_cast<int32_t*>(list + n_pages);
   const cudaStream_t st = as_stream(stream);
   rc = launch_next("paged_extend", extend_kernel, dim3(1), kPlanThreads, 0, st, m, slots, n, n_new,
-                   (int)n_new_all, status, moves, list, pages);
+                   (int)n_new_all, status, moves, list, pages, granted);
   if (rc) return rc;
   return launch_move("paged_extend (copy)", pool, pool, layer_stride, layer_stride, page_bytes,
                      n_layers, moves, list, Renumber{}, st);

@@ -104,6 +104,9 @@ _SIGNATURES = {
     "kvq_paged_append": (_c_int, [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_int, _c_p, _c_int,
                                   _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p,
                                   _c_p, _c_i64, _c_i64, _c_p]),
+    "kvq_paged_append_granted": (_c_int, [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_int, _c_p,
+                                          _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64,
+                                          _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p]),
     "kvq_paged_read": (_c_int, [_c_p, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
                                 _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_int, _c_p]),
     "kvq_paged_attention_workspace": (_c_size, [_c_i64, _c_i64, _c_i64]),
@@ -119,6 +122,9 @@ _SIGNATURES = {
     "kvq_paged_extend": (_c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p,
                                   _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_size,
                                   _c_p]),
+    "kvq_paged_extend_granting": (_c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
+                                           _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_i64,
+                                           _c_p, _c_p, _c_size, _c_p, _c_p]),
     "kvq_paged_compact": (_c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p,
                                    _c_i64, _c_p, _c_p, _c_size, _c_p]),
     "kvq_paged_copy_workspace": (_c_size, [_c_i64]),

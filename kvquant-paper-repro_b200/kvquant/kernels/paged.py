@@ -117,7 +117,8 @@ def _rows(what: str, name: str, t, heads, dim, dev: int):
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, table: torch.Tensor,
                  lengths: torch.Tensor, kind: str, slots: torch.Tensor | None = None,
-                 indptr: torch.Tensor | None = None, max_new: int | None = None) -> None:
+                 indptr: torch.Tensor | None = None, max_new: int | None = None,
+                 granted: torch.Tensor | None = None) -> None:
     """Writes the new tokens' keys and values [N, heads, D] (fp16 or bf16) into their blocks.
 
     A block that the call starts gets the scale max|x| / largest code (at least
@@ -126,6 +127,12 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, table: to
     are rounded to nearest even; infinities are stored as the largest code, NaN as 0,
     and neither counts towards the scale. max_new is accepted for symmetry with
     paged_attention and not needed.
+
+    granted (int32 [slots], kept by paged_extend): sequences whose rows reach before the
+    first token that their slot's last extend granted are skipped and flagged, so that an
+    append after a refused extend leaves what is stored alone. Without it the caller has
+    to know that the extend was not refused: the rows would overwrite the slots' last
+    tokens, in shared pages too.
     """
     what = "paged_append"
     cache, ip, B, heads, dim, dev = _cache_args(what, pool, kind, table, lengths, slots, indptr)
@@ -135,8 +142,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, table: to
     if k.shape != v.shape or k.dtype is not v.dtype or code == 2:
         raise RuntimeError("paged_append: k and v must have one shape and be fp16 or bf16")
     lib = get_cuda_ops().lib
-    _launch(lib.kvq_paged_append, lib, dev, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row,
-            v_head, code, *cache, ip, B, k.shape[0])
+    _launch(lib.kvq_paged_append_granted, lib, dev, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row,
+            v_head, code, *cache, ip, B, k.shape[0],
+            _int32(what, "granted", granted, dev, cache[7]))
 
 
 def paged_read(pool: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, kind: str,
@@ -254,14 +262,16 @@ def paged_fork(table, lengths, refs, src, dst, page_tokens: int, status) -> None
 
 
 def paged_extend(pool, table, lengths, refs, slots, n_new, status,
-                 workspace: DecodeWorkspace | None = None) -> None:
+                 workspace: DecodeWorkspace | None = None,
+                 granted: torch.Tensor | None = None) -> None:
     """Room for n_new (int, or int32 per slot) more tokens in every slot; lengths grow.
 
     Free pages are taken in ascending order, slot after slot. A slot whose last page is
     open and shared gets its own copy of it, in every layer of pool ([layers, ...] or one
     layer's), unless all other holders stand before it in `slots`. When pages run out
     (NO_PAGES in status), or a slot is out of range, named twice or too long for its row
-    (BAD_SLOT), nothing changes.
+    (BAD_SLOT), nothing changes. granted (int32 [slots of the table], for paged_append)
+    gets each slot's first new token, or 2**31 - 1 when the call is refused.
     """
     what = "paged_extend"
     where, pages, page_tokens = _pool_args(what, pool)
@@ -272,9 +282,11 @@ def paged_extend(pool, table, lengths, refs, slots, n_new, status,
     each = isinstance(n_new, torch.Tensor)
     lib = get_cuda_ops().lib
     ws = (workspace or DecodeWorkspace()).get(lib.kvq_paged_extend_workspace(pages), pool.device)
-    _launch(lib.kvq_paged_extend, lib, dev, *where, *meta, _int32(what, "slots", slots, dev), n,
+    _launch(lib.kvq_paged_extend_granting, lib, dev, *where, *meta,
+            _int32(what, "slots", slots, dev), n,
             _int32(what, "n_new", n_new, dev, n) if each else None, 0 if each else n_new,
-            _int32(what, "status", status, dev, 1), ws.data_ptr(), ws.numel())
+            _int32(what, "status", status, dev, 1), ws.data_ptr(), ws.numel(),
+            _int32(what, "granted", granted, dev, meta[1]))
 
 
 def paged_compact(pool, table, refs, workspace: DecodeWorkspace | None = None,

@@ -13,6 +13,11 @@ its calls can be captured in a CUDA graph.
         o = cache.attend(layer, q, slots, indptr)   # causal over everything cached
     cache.fork(src, dst)                            # dst share src's pages (copy-on-write)
     cache.free(slots); cache.compact()
+    cache.check()                                   # RuntimeError if something was refused
+
+append writes only tokens that the slot's last extend granted. When an extend is refused
+(no free pages, a bad slot), the appends of its slots write nothing until an extend of theirs
+is granted, and their attend sees the tokens stored before.
 """
 from __future__ import annotations
 
@@ -46,6 +51,8 @@ class PagedKVCache:
         self.lengths = torch.zeros(max_slots, **ints)
         self.refs = torch.zeros(n_pages, **ints)
         self.status = torch.zeros(1, **ints)
+        # the first token that a slot's last extend granted; none yet
+        self.granted = torch.full((max_slots,), 2 ** 31 - 1, **ints)
         self.workspace = DecodeWorkspace()  # one stream at a time
 
     def _slots(self, slots):
@@ -57,7 +64,7 @@ class PagedKVCache:
     def extend(self, slots, n_new) -> None:
         """Room for n_new (int, or int32 tensor) more tokens in each of the slots."""
         paged_extend(self.pool, self.table, self.lengths, self.refs, self._slots(slots), n_new,
-                     self.status, workspace=self.workspace)
+                     self.status, workspace=self.workspace, granted=self.granted)
 
     def fork(self, src, dst) -> None:
         """dst[i] (empty) becomes a copy of src[i] that shares its pages."""
@@ -80,13 +87,15 @@ class PagedKVCache:
         if s:
             self.status.zero_()
             why = [t for bit, t in ((NO_PAGES, "no free pages"), (BAD_SLOT, "a bad slot")) if s & bit]
-            raise RuntimeError(f"PagedKVCache: {' and '.join(why)}; nothing was changed for it")
+            raise RuntimeError(f"PagedKVCache: {' and '.join(why)}; nothing was changed for it "
+                               "and its tokens were not written")
 
     # -- tokens -------------------------------------------------------------------
     def append(self, layer: int, k, v, slots=None, indptr=None) -> None:
-        """Writes the new tokens' keys and values [N, heads, D]: the last ones of the slots."""
+        """Writes the new tokens' keys and values [N, heads, D]: the last ones of the slots, as
+        far as their last extend granted them."""
         paged_append(k, v, self.pool[layer], self.table, self.lengths, self.kind,
-                     slots=self._slots(slots), indptr=indptr)
+                     slots=self._slots(slots), indptr=indptr, granted=self.granted)
 
     def attend(self, layer: int, q, slots=None, indptr=None, max_new=None, **kw):
         """Causal attention of the new tokens' queries [N, Hq, D] (see paged_attention)."""
