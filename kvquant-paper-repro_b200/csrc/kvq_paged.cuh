@@ -682,12 +682,14 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Meta m, const int3
                                                               int n_new_all, int32_t* status,
                                                               Moves* moves, int2* list,
                                                               int32_t* pages, int32_t* granted) {
+  static_assert(kPlanThreads == 32 * 32, "a warp holds one sum of every warp");
   wait_previous();
   let_next_start();
   __shared__ int warp_sums[32];
   __shared__ int last_page[kMaxSeqs];  // shared open page of slot i, or -1 - i
   __shared__ int need[kMaxSeqs];       // pages, then its offset; copy flag in `copies`
   __shared__ uint8_t copies[kMaxSeqs];
+  __shared__ int64_t warp_asked[32];
   const int tid = threadIdx.x;
   auto refuse = [&](int why) {
     for (int64_t i = tid; granted && i < n; i += kPlanThreads)
@@ -719,6 +721,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Meta m, const int3
     }
   }
   bad = __syncthreads_or(bad);
+  int64_t asked = 0;  // pages of all slots; the 32-bit sums below hold up to n_pages
   for (int i = tid; i < n; i += kPlanThreads) {
     const int s = slots[i], p = last_page[i];
     int before = 0;
@@ -729,10 +732,17 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Meta m, const int3
     const bool copy = p >= 0 && m.refs[p] - before > 1;
     copies[i] = copy;
     need[i] += copy;
+    asked += need[i];
   }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) asked += __shfl_xor_sync(0xffffffffu, asked, o);
+  warp_asked[tid >> 5] = asked;
   bad = __syncthreads_or(bad);
-  if (bad) {
-    refuse(kBadSlot);
+  asked = warp_asked[tid & 31];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) asked += __shfl_xor_sync(0xffffffffu, asked, o);
+  if (bad || asked > m.n_pages) {
+    refuse(bad ? kBadSlot : kNoPages);
     return;
   }
   int total = 0;

@@ -43,3 +43,22 @@ def test_copy_of_many_pages(cuda, n):
     b[:, dst[~bad]] = a[:, src[~bad]]
     np.testing.assert_array_equal(gb.cpu().numpy(), b)
     np.testing.assert_array_equal(ga.cpu().numpy(), a)
+
+
+def test_extend_by_more_pages_than_32_bits_count(cuda):
+    """17 slots of 134217727 pages each: their sum is past 2**31. The call is refused and the
+    table (9 GB) stays as it is."""
+    from kvquant.kernels import paged_extend
+    from kvquant.kernels.paged import NO_PAGES, pool_shape
+    ints = dict(dtype=torch.int32, device=cuda)
+    n, cols = 17, (2 ** 31 - 1) // 16
+    pool = torch.zeros(pool_shape(8, 1, 64, 16), dtype=torch.uint8, device=cuda)
+    table = torch.full((n, cols), -1, **ints)
+    lengths, refs, status = torch.zeros(n, **ints), torch.zeros(8, **ints), torch.zeros(1, **ints)
+    slots = torch.arange(n, **ints)
+    paged_extend(pool, table, lengths, refs, slots, torch.full((n,), 16 * cols, **ints), status)
+    assert int(status.item()) == NO_PAGES
+    assert int(table.max().item()) == -1 and int(table.min().item()) == -1
+    assert not lengths.any() and not refs.any()
+    paged_extend(pool, table, lengths, refs, slots[:8], 16, status)
+    assert torch.equal(table[:8, 0], slots[:8]) and refs.eq(1).all() and lengths[:8].eq(16).all()
