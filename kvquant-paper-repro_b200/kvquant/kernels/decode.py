@@ -379,7 +379,9 @@ def set_decode_kernels(key: str | None = None, value: str | None = None) -> tupl
 
 
 class DecodeWorkspace:
-    """Reusable scratch for decode_attention (one per stream)."""
+    """Reusable scratch for decode_attention and the paged calls (one per stream). A call that
+    needs more than those before replaces the buffer: capture calls in a CUDA graph only once
+    the largest one has run, or give the graph a workspace of its own."""
 
     def __init__(self):
         self.buf = None

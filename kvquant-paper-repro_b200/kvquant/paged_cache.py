@@ -25,6 +25,7 @@ import torch
 
 from .kernels import (DecodeWorkspace, paged_append, paged_attention, paged_compact,
                       paged_extend, paged_fork, paged_free, paged_read)
+from .kernels.cuda_ops import get_cuda_ops
 from .kernels.paged import BAD_SLOT, KINDS, NO_PAGES, pool_shape
 
 
@@ -53,7 +54,13 @@ class PagedKVCache:
         self.status = torch.zeros(1, **ints)
         # the first token that a slot's last extend granted; none yet
         self.granted = torch.full((max_slots,), 2 ** 31 - 1, **ints)
-        self.workspace = DecodeWorkspace()  # one stream at a time
+        # One stream at a time. As large as any call needs (20 or 40 MB at head_dim 64 or 128):
+        # a buffer that grew would leave captured calls with an address that is given back.
+        lib = get_cuda_ops().lib
+        self.workspace = DecodeWorkspace()
+        self.workspace.get(max(lib.kvq_paged_extend_workspace(n_pages),
+                               *(lib.kvq_paged_attention_workspace(head_dim, n, 1)
+                                 for n in (1, 48, 65536))), self.pool.device)
 
     def _slots(self, slots):
         if slots is None or isinstance(slots, torch.Tensor):
