@@ -405,8 +405,8 @@ int kvq_paged_read(const uint8_t* pool, int kind, int64_t n_pages, int64_t n_hea
  * D] in q's type; a row at position p sees the tokens j <= p, with window > 0
  * only j > p - window; a row that sees none is 0. ml_out: NULL or fp32 pairs
  * [total, n_heads * group] = (M, 1 / L) of softmax(scores * scale), (-inf, inf)
- * for such a row (kvq_merge_shards takes them). group <= 64; max_new: the most
- * rows of any sequence (a sequence with more is skipped and flagged). */
+ * for such a row (kvq_merge_shards takes them). group <= 64; max_new (up to 65536):
+ * the most rows of any sequence (a sequence with more is skipped and flagged). */
 size_t kvq_paged_attention_workspace(int64_t head_dim, int64_t max_new, int64_t group);
 int kvq_paged_attention(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int dtype,
                         int64_t group, const uint8_t* pool, int kind, int64_t n_pages,

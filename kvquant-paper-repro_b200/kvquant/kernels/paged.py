@@ -31,6 +31,7 @@ from .cuda_ops import _check, _ptr, get_cuda_ops
 from .decode import DecodeWorkspace
 
 BLOCK_TOKENS = 16
+MAX_NEW = 65536  # most rows of one sequence in a call of paged_attention
 KINDS = {"int8": 0, "e4m3": 1}
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
@@ -178,8 +179,10 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor,
     see nothing are 0. ml_out (fp32 [N, Hq, 2], optional) receives each row's softmax
     statistics (M, 1/L) of softmax(scores * scale), (-inf, inf) for such rows: with
     the fp16 outputs merge_shards joins them with other parts of the same context.
-    max_new: the most rows of any sequence (default: N when indptr is given; a smaller
-    bound gives a better split); scale defaults to 1 / sqrt(D).
+    max_new: the most rows of any sequence, at most 65536 (a sequence with more is skipped and
+    flagged). Give it with indptr: it also picks the kernel, and the default there, N or
+    65536 if N is more, takes a batch of single tokens for one prompt chunk and pads every
+    sequence to 256 rows. scale defaults to 1 / sqrt(D).
     """
     what = "paged_attention"
     cache, ip, B, heads, dim, dev = _cache_args(what, pool, kind, table, lengths, slots, indptr)
@@ -199,7 +202,7 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, table: torch.Tensor,
                                or ml_out.numel() != N * Hq * 2 or ml_out.get_device() != dev):
         raise RuntimeError("paged_attention: ml_out must be contiguous fp32 [N, Hq, 2]")
     if max_new is None:
-        max_new = N if indptr is not None else N // max(1, B)
+        max_new = min(N, MAX_NEW) if indptr is not None else N // max(1, B)
     lib = get_cuda_ops().lib
     need = lib.kvq_paged_attention_workspace(dim, max_new, Hq // heads)
     ws = (workspace or DecodeWorkspace()).get(need, pool.device)

@@ -10,7 +10,7 @@ its calls can be captured in a CUDA graph.
     cache.extend(slots, n_new)                      # room for the new tokens; lengths grow
     for layer in range(32):
         cache.append(layer, k, v, slots, indptr)    # the new tokens' rotated keys, values
-        o = cache.attend(layer, q, slots, indptr)   # causal over everything cached
+        o = cache.attend(layer, q, slots, indptr, max_new=most)  # causal over everything cached
     cache.fork(src, dst)                            # dst share src's pages (copy-on-write)
     cache.free(slots); cache.compact()
     cache.check()                                   # RuntimeError if something was refused
@@ -105,7 +105,8 @@ class PagedKVCache:
                      slots=self._slots(slots), indptr=indptr, granted=self.granted)
 
     def attend(self, layer: int, q, slots=None, indptr=None, max_new=None, **kw):
-        """Causal attention of the new tokens' queries [N, Hq, D] (see paged_attention)."""
+        """Causal attention of the new tokens' queries [N, Hq, D]. With indptr give max_new, the
+        most rows of any slot (see paged_attention)."""
         return paged_attention(q, self.pool[layer], self.table, self.lengths, self.kind,
                                slots=self._slots(slots), indptr=indptr, max_new=max_new,
                                workspace=self.workspace, **kw)

@@ -62,3 +62,21 @@ def test_extend_by_more_pages_than_32_bits_count(cuda):
     assert not lengths.any() and not refs.any()
     paged_extend(pool, table, lengths, refs, slots[:8], 16, status)
     assert torch.equal(table[:8, 0], slots[:8]) and refs.eq(1).all() and lengths[:8].eq(16).all()
+
+
+def test_more_rows_than_any_sequence_may_have(cuda):
+    """80000 rows of 40 prompts, without max_new: no sequence is near the limit of 65536."""
+    from kvquant.kernels import paged_attention
+    from kvquant.kernels.cuda_ops import get_cuda_ops
+    c = Cache([2000], H=1, D=64, page=64, seed=22)
+    pool, table, lengths = c.gpu(cuda)
+    table, lengths = table.repeat(40, 1), lengths.repeat(40)  # the same pages for all
+    q = torch.from_numpy(c.queries([2000], 1)).to(cuda).half().repeat(40, 1, 1)
+    ip = torch.arange(0, 80001, 2000, dtype=torch.int32, device=cuda)
+    got = paged_attention(q, pool, table, lengths, "int8", indptr=ip)
+    get_cuda_ops().check_status(cuda)
+    want = paged_attention(q, pool, table, lengths, "int8", indptr=ip, max_new=2000)
+    assert torch.equal(got, want)
+    out, _, bound, _ = expected(c, q[:2000].float().cpu().numpy(), [2000], 1)
+    for i in (0, 17, 39):
+        check(got[2000 * i:2000 * (i + 1)].float().cpu().numpy(), out, bound, f"prompt {i}")
