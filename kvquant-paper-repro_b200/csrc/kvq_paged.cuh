@@ -578,8 +578,7 @@ struct Meta {
   int64_t n_slots, n_cols;
   int32_t* lengths;
   int32_t* refs;
-  int64_t n_pages;
-  int page_tokens;
+  int64_t n_pages, page_tokens;
 };
 
 constexpr int kPageThreads = 256;
@@ -947,7 +946,7 @@ static int launch_next(const char* what, void (*kernel)(Params...), dim3 grid, i
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-inline int check_view(const char* what, const View& v, int kind, int page_tokens) {
+inline int check_view(const char* what, const View& v, int kind, int64_t page_tokens) {
   if (v.dim != 64 && v.dim != 128) {
     set_error("%s: head_dim must be 64 or 128 (got %d)", what, v.dim);
     return KVQ_ERR_UNSUPPORTED;
@@ -957,7 +956,8 @@ inline int check_view(const char* what, const View& v, int kind, int page_tokens
     return KVQ_ERR_UNSUPPORTED;
   }
   if (page_tokens < kBlock || page_tokens > 1024 || page_tokens % kBlock) {
-    set_error("%s: page_tokens must be a multiple of 16 in 16..1024 (got %d)", what, page_tokens);
+    set_error("%s: page_tokens must be a multiple of 16 in 16..1024 (got %lld)", what,
+              (long long)page_tokens);
     return KVQ_ERR_INVALID;
   }
   if (v.n_pages < 1 || v.n_pages > INT32_MAX || v.heads < 1 || v.heads > 1024 || v.n_slots < 1 ||
@@ -987,8 +987,9 @@ inline int check_meta(const char* what, const Meta& m) {
   if (!m.table || !m.refs || m.n_slots < 1 || m.n_slots > INT32_MAX || m.n_cols < 1 ||
       m.n_pages < 1 || m.n_pages > INT32_MAX || m.page_tokens < kBlock ||
       m.page_tokens % kBlock || m.n_cols > INT32_MAX / m.page_tokens) {
-    set_error("%s: invalid table (%lld x %lld), counts (%lld pages) or page size %d", what,
-              (long long)m.n_slots, (long long)m.n_cols, (long long)m.n_pages, m.page_tokens);
+    set_error("%s: invalid table (%lld x %lld), counts (%lld pages) or page size %lld", what,
+              (long long)m.n_slots, (long long)m.n_cols, (long long)m.n_pages,
+              (long long)m.page_tokens);
     return KVQ_ERR_INVALID;
   }
   return KVQ_OK;
@@ -1048,7 +1049,7 @@ inline size_t plan_bytes(int64_t n_pages) {
 
 inline int check_pool(const char* what, const uint8_t* pool, int64_t n_layers, int64_t page_bytes) {
   if (!pool || !aligned16(pool) || n_layers < 1 || n_layers > INT32_MAX || page_bytes < 16 ||
-      page_bytes % 16) {
+      page_bytes % 16 || page_bytes > INT64_MAX / INT32_MAX) {
     set_error("%s: the pool must be 16-byte aligned with whole records (%lld layers, %lld bytes "
               "a page)", what, (long long)n_layers, (long long)page_bytes);
     return KVQ_ERR_INVALID;
@@ -1085,7 +1086,7 @@ extern "C" int kvq_paged_append_granted(const void* k, int64_t k_tok_stride, int
   clear_error();
   const View w = make_view(pool, n_pages, n_heads, head_dim, page_tokens, table, n_slots, n_cols,
                            lengths, slots, indptr, B, total);
-  int rc = check_view("paged_append", w, kind, (int)page_tokens);
+  int rc = check_view("paged_append", w, kind, page_tokens);
   if (rc) return rc;
   if (dtype != 0 && dtype != 1) {
     set_error("paged_append: dtype must be 0 (fp16) or 1 (bf16), got %d", dtype);
@@ -1125,7 +1126,7 @@ extern "C" int kvq_paged_read(const uint8_t* pool, int kind, int64_t n_pages, in
   clear_error();
   const View w = make_view(const_cast<uint8_t*>(pool), n_pages, n_heads, head_dim, page_tokens,
                            table, n_slots, n_cols, lengths, slots, indptr, B, total);
-  int rc = check_view("paged_read", w, kind, (int)page_tokens);
+  int rc = check_view("paged_read", w, kind, page_tokens);
   if (rc) return rc;
   if (dtype < 0 || dtype > 2) {
     set_error("paged_read: dtype must be 0 (fp16), 1 (bf16) or 2 (fp32), got %d", dtype);
@@ -1160,7 +1161,7 @@ extern "C" int kvq_paged_free(int32_t* table, int64_t n_slots, int64_t n_cols, i
   using namespace kvq;
   using namespace kvq::paged;
   clear_error();
-  const Meta m{table, n_slots, n_cols, lengths, refs, n_pages, (int)page_tokens};
+  const Meta m{table, n_slots, n_cols, lengths, refs, n_pages, page_tokens};
   int rc = check_meta("paged_free", m);
   if (rc) return rc;
   if (n < 0 || n > kMaxSeqs || !lengths || !status || (n && !slots)) {
@@ -1179,7 +1180,7 @@ extern "C" int kvq_paged_fork(int32_t* table, int64_t n_slots, int64_t n_cols, i
   using namespace kvq;
   using namespace kvq::paged;
   clear_error();
-  const Meta m{table, n_slots, n_cols, lengths, refs, n_pages, (int)page_tokens};
+  const Meta m{table, n_slots, n_cols, lengths, refs, n_pages, page_tokens};
   int rc = check_meta("paged_fork", m);
   if (rc) return rc;
   if (n < 0 || n > kMaxSeqs || !lengths || !status || (n && (!src || !dst))) {
@@ -1216,7 +1217,7 @@ extern "C" int kvq_paged_extend_granting(uint8_t* pool, int64_t n_layers, int64_
   using namespace kvq;
   using namespace kvq::paged;
   clear_error();
-  const Meta m{table, n_slots, n_cols, lengths, refs, n_pages, (int)page_tokens};
+  const Meta m{table, n_slots, n_cols, lengths, refs, n_pages, page_tokens};
   int rc = check_meta("paged_extend", m);
   if (!rc) rc = check_pool("paged_extend", pool, n_layers, page_bytes);
   if (rc) return rc;
@@ -1302,8 +1303,10 @@ extern "C" int kvq_paged_copy(const uint8_t* src_pool, int64_t src_pages,
   if (rc) return rc;
   if (n < 0 || n > INT32_MAX || (n && (!src || !dst)) || src_pages < 1 || dst_pages < 1 ||
       src_pages > INT32_MAX || dst_pages > INT32_MAX || src_layer_stride % 16 ||
-      dst_layer_stride % 16) {
-    set_error("paged_copy: invalid pairs (%lld), pools (%lld, %lld pages) or strides",
+      dst_layer_stride % 16 ||
+      (n_layers > 1 && (src_layer_stride < src_pages * page_bytes ||
+                        dst_layer_stride < dst_pages * page_bytes))) {
+    set_error("paged_copy: invalid pairs (%lld), pools (%lld, %lld pages) or layer strides",
               (long long)n, (long long)src_pages, (long long)dst_pages);
     return KVQ_ERR_INVALID;
   }

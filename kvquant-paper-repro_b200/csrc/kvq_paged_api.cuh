@@ -36,7 +36,7 @@ extern "C" int kvq_paged_attention(const void* q, int64_t q_tok_stride, int64_t 
   AttnArgs a;
   a.v = make_view(const_cast<uint8_t*>(pool), n_pages, n_heads, head_dim, page_tokens, table,
                   n_slots, n_cols, lengths, slots, indptr, B, total);
-  int rc = check_view("paged_attention", a.v, kind, (int)page_tokens);
+  int rc = check_view("paged_attention", a.v, kind, page_tokens);
   if (rc) return rc;
   if (dtype != 0 && dtype != 1) {
     set_error("paged_attention: dtype must be 0 (fp16) or 1 (bf16), got %d", dtype);
