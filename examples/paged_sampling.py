@@ -110,6 +110,7 @@ def main(argv=None):
     cache.fork(src, live)
     dense.fork(src, live)
     cache.free(list(range(n_p)))  # the prompts' own slots; the samples hold their pages
+    n_live = cache.compact()
     x = x[(ints(prompts).cumsum(0) - 1).long()].repeat_interleave(args.samples, 0)
     for i in range(args.steps):
         x = step(x + 0.3 * torch.randn_like(x), live, [1] * len(live))

@@ -96,3 +96,12 @@ def test_append_only_where_extend_granted(cuda):
     get_cuda_ops().check_status(cuda)
     assert not torch.equal(c.pool, before)
     c.check()
+
+
+def test_example_without_steps(cuda):
+    """The example with nothing but its prompts."""
+    import sys
+    from pathlib import Path
+    sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "examples"))
+    import paged_sampling
+    assert paged_sampling.main(["--steps", "0", "--samples", "2"]) < 0.02
