@@ -364,6 +364,8 @@ int kvq_decode_kernels(void);
  *            tokens (lengths already counts them).
  * Pages, slots, lengths and row ranges that are out of range are skipped and
  * make kvq_check_status() fail; nothing outside the given arrays is touched.
+ * Output rows of a skipped sequence, and rows that indptr gives to none, keep
+ * what they held.
  * dtype: 0 = fp16, 1 = bf16, 2 = fp32 (outputs of kvq_paged_read only).
  * Strides are in elements.
  * ------------------------------------------------------------------------- */

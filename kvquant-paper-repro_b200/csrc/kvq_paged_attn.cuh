@@ -380,8 +380,8 @@ __device__ __forceinline__ float2 row_stats(float m, float ref, float l) {
 
 // 8 consumer warps, and 4 that feed two each. A copy is issued for one lane at a time
 // (~190 cycles each), so one warp that fed all eight was what bound the kernel: 1500
-// cycles for 8 records, the rate of HBM itself (262144 tokens x 32 heads: 370 us with
-// one, 315 with four).
+// cycles for 8 records, the rate of HBM itself (262144 tokens x 32 heads, passes of a
+// graph: 370 us with one, 315 with four).
 constexpr int kAttnWarps = 8, kFeeds = 2;
 constexpr int kAttnThreads = 32 * (kAttnWarps + kAttnWarps / kFeeds);
 constexpr int kSms = 148;
@@ -438,10 +438,12 @@ struct Cursor {
 // One CTA per SM. Every consumer warp works through its own share of the blocks
 // with its own ring of records, so no warp waits for another one; a lane of a
 // feeding warp keeps each ring full: one bulk copy per record, on across the ends of
-// units. Bound by HBM: 262144 tokens x 32 heads, 2.16 GB, take 315 us = 6.8 TB/s (of a
-// measured copy rate of 6.55); 16 sequences of up to 8192, 0.145 GB, 37 us, of which
-// ~7 pass before the first record, ~5 in the join, and the last SM ends ~5 after the
-// median one.
+// units. Bound by HBM: 262144 tokens x 32 heads, 2.16 GB, take 316 us once 512 MB of
+// something else have been read (6.8 TB/s; a copy, which writes as much as it reads,
+// measures 6.55), 347 after 512 MB have been written, 322 to 357 a call in long runs of
+// them; 16 sequences of up to 8192, 0.145 GB, 37 us, of which ~7 pass before the first
+// record, ~5 in the join, and the last SM ends ~5 after the median one. 16 rows at D = 128
+// spill about 200 bytes a thread (168 registers), 8 rows nothing.
 template <int D, int KIND, int NT, typename T>
 __global__ void __launch_bounds__(kAttnThreads, 1) attend_kernel(AttnArgs a) {
   constexpr int R = 8 * NT, S = Ring<D>::kStages;

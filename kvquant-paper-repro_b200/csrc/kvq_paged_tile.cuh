@@ -14,11 +14,12 @@
 // a warp writes whole 128-byte core matrices without bank conflicts.
 // One CTA per SM takes an equal share of all (unit, token tile) pairs; a unit
 // cut by a share's end is joined by tile_join_kernel. Two chunks of 2048 tokens x 4
-// heads over 8200 and 10007 tokens, 8 KV heads: 728 us = 0.80 PFLOP/s, 48 % of the
-// measured bf16 rate. A token tile takes 5300 cycles: a tile's softmax ~3300 (MUFU
-// 1024, two warps to a partition) and then its 16 products ~1900 follow each other,
-// and the two tiles overlap only in part. Two issuing warps, one per tile, were
-// slower (951 us): their products interleave and both softmaxes fall together.
+// heads over 8200 and 10007 tokens, 8 KV heads: 754 us = 0.78 PFLOP/s, 47 % of the
+// measured bf16 rate. A token tile takes about 5500 cycles: a tile's softmax ~3300 and
+// its rescalings of O (MUFU 1024, two warps to a partition) and then its 16 products ~1900
+// follow each other, and the two tiles overlap only in part. Two issuing warps, one per
+// tile, were slower (951 us against 725 then): their products interleave and both
+// softmaxes fall together. About 110 bytes a thread spill.
 #pragma once
 #include "kvq_paged_attn.cuh"
 

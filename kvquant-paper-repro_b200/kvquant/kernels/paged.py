@@ -21,7 +21,8 @@ A slot appears at most once in a call.
 
 All tensors are CUDA tensors; work is launched on the current stream. Page ids,
 slots and row ranges that are out of range are skipped and reported by
-get_cuda_ops().check_status().
+get_cuda_ops().check_status(); output rows of a skipped sequence, and rows that indptr gives
+to none, are not written.
 """
 from __future__ import annotations
 

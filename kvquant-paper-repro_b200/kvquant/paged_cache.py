@@ -4,7 +4,8 @@ QuantizedKVCache holds one slot per layer, kvquant/kv_cache.py:12-32).
 A slot is one sequence. Its pages are shared by all layers: page p of layer l is
 pool[l, p]. Table, lengths and reference counts live on the device and only kernels
 change them, so a decode loop neither synchronises nor copies them to the host, and
-its calls can be captured in a CUDA graph.
+its calls can be captured in a CUDA graph. (Slots as int32 tensors: a Python list is
+copied to the device by every call that gets it, which waits for the copy.)
 
     cache = PagedKVCache(n_layers=32, n_pages=4096, heads=8, max_slots=64, max_tokens=8192)
     cache.extend(slots, n_new)                      # room for the new tokens; lengths grow
